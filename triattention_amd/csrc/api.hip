@@ -15,9 +15,11 @@
 #include "../../include/triattention_amd.h"
 #include "cache.hip"
 #include "decode.hip"
+#include "linear.hip"
 #include "prefill.hip"
 #include "probe.hip"
 #include "quantize.hip"
+#include "rows.hip"
 #include "tail.hip"
 
 namespace {
@@ -960,6 +962,130 @@ int tri_issue_probe(int mode, int waves_per_simd, int iters, int64_t* out, void*
   hipLaunchKernelGGL(kernels[mode], dim3(cus), dim3(256 * waves_per_simd), LDS, static_cast<hipStream_t>(stream), iters,
                      out, 1.0001f, 0.5f, 3);
   return check_launch("issue_probe");
+}
+
+static int row_args(tri::RowArgs& a, const char* what, const void* x, int64_t ldx, int dtype, int64_t m, int64_t k,
+                    int8_t* codes, int64_t ldc, float* scales) {
+  if (m < 0 || k < 1 || k > INT32_MAX - 65536) return fail("%s: rows of 1 to 2^31 - 65537 elements", what);
+  if (dtype < 0 || dtype > 2) return fail("%s: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)", what);
+  if (m > 0 && (!x || !codes || !scales)) return fail("%s: null buffer", what);
+  if (ldx < 0 || (m > 1 && ldc < k)) return fail("%s: row strides (codes rows may not overlap)", what);
+  a.x = x;
+  a.ldx = ldx;
+  a.m = m;
+  a.k = (int)k;
+  a.codes = codes;
+  a.ldc = ldc;
+  a.scales = scales;
+  return 0;
+}
+
+int tri_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t m, int64_t k, int8_t* codes, int64_t ldc,
+                      float* scales, void* stream) {
+  g_error.clear();
+  tri::RowArgs a{};
+  if (row_args(a, "quantize_rows", x, ldx, dtype, m, k, codes, ldc, scales)) return 1;
+  if (m == 0) return 0;
+  tri::launch_rows<tri::ROWS>(a, dtype, static_cast<hipStream_t>(stream));
+  return check_launch("quantize_rows");
+}
+
+int tri_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int dtype,
+                       int64_t m, int64_t k, double eps, int8_t* codes, int64_t ldc, float* scales, void* hidden,
+                       int64_t ldh, void* stream) {
+  g_error.clear();
+  tri::RowArgs a{};
+  if (row_args(a, "rms_norm_quant", x, ldx, dtype, m, k, codes, ldc, scales)) return 1;
+  a.eps = (float)eps;
+  if (!(a.eps >= 1.17549435e-38f) || !std::isfinite(a.eps)) return fail("rms_norm_quant: eps must be positive (a normal fp32 number)");
+  if (m == 0) return 0;
+  if (!weight) return fail("rms_norm_quant: null buffer");
+  if ((residual == nullptr) != (hidden == nullptr)) return fail("rms_norm_quant: residual and hidden (both or neither)");
+  if (residual && (ldr < 0 || (m > 1 && ldh < k))) return fail("rms_norm_quant: row strides (hidden rows may not overlap)");
+  a.r = residual;
+  a.ldr = ldr;
+  a.w = weight;
+  a.hidden = hidden;
+  a.ldh = ldh;
+  tri::launch_rows<tri::NORM>(a, dtype, static_cast<hipStream_t>(stream));
+  return check_launch("rms_norm_quant");
+}
+
+int tri_silu_mul_quant(const void* gate, int64_t ldg, const void* up, int64_t ldu, int dtype, int64_t m, int64_t k,
+                       int8_t* codes, int64_t ldc, float* scales, void* stream) {
+  g_error.clear();
+  tri::RowArgs a{};
+  if (row_args(a, "silu_mul_quant", gate, ldg, dtype, m, k, codes, ldc, scales)) return 1;
+  if (m == 0) return 0;
+  if (!up) return fail("silu_mul_quant: null buffer");
+  if (ldu < 0) return fail("silu_mul_quant: row strides");
+  a.r = up;
+  a.ldr = ldu;
+  tri::launch_rows<tri::SILU>(a, dtype, static_cast<hipStream_t>(stream));
+  return check_launch("silu_mul_quant");
+}
+
+static int linear_shape(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 1 || k < 1) return fail("int8_linear: empty shape");
+  if (k > tri::LIN_MAX_K) return fail("int8_linear: at most %d input channels (int32 sums)", tri::LIN_MAX_K);
+  if (m > (1 << 30) || n > (1 << 30)) return fail("int8_linear: at most 2^30 rows and output channels");
+  return 0;
+}
+
+int tri_int8_linear_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes) {
+  g_error.clear();
+  if (!bytes) return fail("int8_linear: null output");
+  *bytes = 0;
+  if (linear_shape(m, n, k)) return 1;
+  int cus = 0;
+  if (m == 0) return 0;
+  if (device_cus(&cus)) return 1;
+  const tri::LinearPlan p = tri::linear_plan((int)m, (int)n, (int)k, cus);
+  if (p.splits > 1) *bytes = p.splits * m * n * 4;
+  return 0;
+}
+
+int tri_int8_linear(const int8_t* x, int64_t ldx, const float* xs, const int8_t* w, int64_t ldw, const float* ws,
+                    const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo, int dtype, int64_t m,
+                    int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream) {
+  g_error.clear();
+  if (linear_shape(m, n, k)) return 1;
+  if (dtype < 0 || dtype > 2) return fail("int8_linear: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  if (m == 0) return 0;
+  if (!x || !xs || !w || !ws || !out) return fail("int8_linear: null buffer");
+  if (!aligned(x, 16) || !aligned(w, 16) || ldx % 16 != 0 || ldw % 16 != 0)
+    return fail("int8_linear: rows of codes must be 16-byte aligned (base and row stride)");
+  if (ldx < 0 || ldx > tri::LIN_MAX_LD || ldw < 0 || ldw > tri::LIN_MAX_LD)
+    return fail("int8_linear: row strides of codes must be at most 4 MiB");
+  if ((m > 1 && ldo < n) || (residual && ldr < 0)) return fail("int8_linear: row strides (output rows may not overlap)");
+  int cus = 0;
+  if (device_cus(&cus)) return 1;
+  const tri::LinearPlan p = tri::linear_plan((int)m, (int)n, (int)k, cus);
+  tri::LinearArgs a{};
+  if (p.splits > 1) {
+    if (!workspace || workspace_bytes < p.splits * m * n * 4 || !aligned(workspace, 16))
+      return fail("int8_linear: workspace too small (%lld bytes needed)", (long long)(p.splits * m * n * 4));
+    a.part = static_cast<int32_t*>(workspace);
+  }
+  if (p.kind && ((m + p.bm - 1) / p.bm) * ((n + p.bn - 1) / p.bn) > (1 << 22))
+    return fail("int8_linear: too many outputs for one call");
+  a.x = x;
+  a.ldx = ldx;
+  a.xs = xs;
+  a.w = w;
+  a.ldw = ldw;
+  a.ws = ws;
+  a.bias = bias;
+  a.residual = residual;
+  a.ldr = ldr;
+  a.out = out;
+  a.ldo = ldo;
+  a.dtype = dtype;
+  a.m = (int)m;
+  a.n = (int)n;
+  a.k = (int)k;
+  tri::launch_linear(a, p, static_cast<hipStream_t>(stream));
+  return check_launch("int8_linear");
 }
 
 }  // extern "C"

@@ -1,0 +1,263 @@
+// Row quantizers of the 8-bit layer: each row of y as int8 codes and one fp32 scale,
+//
+//   a = max_k |y_k|,  s = max(a, 2^-118) / 127,  c_k = rint(y_k * 127 / max(a, 2^-118))    (half to even)
+//
+// with y = x (ROWS), y = h * rsqrt(mean(h^2) + eps) * w with h = x + residual rounded to x's type (NORM: the
+// rounded h is what the next reader of the residual stream sees, so the norm is taken of it), or
+// y = g / (1 + exp(-g)) * u (SILU).  y, the sum of squares and the maximum stay in fp32; the code is the one
+// rounding.  A row whose y or sum of squares is not finite gets scale NaN and codes 0, so that whatever is computed
+// from it is NaN.  The floor 2^-118 keeps 127 / a finite; an all-zero row gets codes 0 and a normal scale.
+//
+// One pass: a row lives in the registers of its threads (T threads, NV vectors of 8 elements each) between the
+// maximum and the codes; NORM needs its sum and its maximum in one reduction, because max |y| = rsqrt(..) * max |h w|.
+// Rows past 32768 elements (NV = 0) are read twice.  Bound by HBM for many rows, by launch and load latency for few.
+#pragma once
+#include "common.h"
+
+namespace tri {
+
+enum RowOp { ROWS = 0, NORM = 1, SILU = 2 };
+enum Dtype { F32 = 0, BF16 = 1, F16 = 2 };
+constexpr float ROW_TINY = 0x1p-118f;
+constexpr int ROW_REGS = 32768;  // longest row held in registers
+
+struct RowArgs {
+  const void* x;         // x or gate
+  const void* r;         // residual (may be null) or up
+  const void* w;         // NORM: weight [k]
+  int64_t ldx, ldr;      // row strides, elements
+  int8_t* codes;
+  int64_t ldc;
+  float* scales;
+  void* hidden;          // NORM with a residual: h [m][ldh]
+  int64_t ldh;
+  int64_t m;             // rows of this launch
+  int k;
+  float eps;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) { return bf16f(v); }
+template <>
+__device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return (float)v; }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16(v); }
+template <>
+__device__ __forceinline__ _Float16 from_f32<_Float16>(float v) { return (_Float16)v; }
+
+// Elements k0 .. k0+7 of a row (0 past the row's end).  The vector access may be unaligned (rows of odd lengths or
+// strides): global memory takes it at the cost of split cache lines.
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int k0, int k, float (&v)[8]) {
+  if (k0 + 8 <= k) {
+    T t[8];
+    __builtin_memcpy(t, row + k0, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k0 + i < k ? to_f32<T>(row[k0 + i]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* __restrict__ row, int k0, int k, const T (&t)[8]) {
+  if (k0 + 8 <= k) {
+    __builtin_memcpy(row + k0, t, sizeof(t));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i < k) row[k0 + i] = t[i];
+  }
+}
+
+// g / (1 + exp(-g)).  exp(-g) = 2^t with t = -g log2(e) held as a rounded product and its error (an fma each), so
+// the relative error stays near an ulp of exp2 for large |g| too; exp(-g) = inf gives -0.
+__device__ __forceinline__ float silu(float g) {
+  constexpr float L2E = 1.44269504f, L2E_LO = 1.92596299e-8f, LN2 = 0.693147181f;
+  const float t = -g * L2E;
+  const float lo = __builtin_fmaf(-g, L2E_LO, __builtin_fmaf(-g, L2E, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  const float ec = e < 3.0e38f ? __builtin_fmaf(e, lo * LN2, e) : e;
+  return g * __builtin_amdgcn_rcpf(1.0f + ec);
+}
+
+// y (NORM: h * w, still without the row's factor) of 8 elements; ss gathers h^2.
+template <int OP, typename T>
+__device__ __forceinline__ void row_values(const RowArgs& a, int64_t row, int k0, float (&y)[8], float& ss, bool write) {
+  load8<T>(static_cast<const T*>(a.x) + row * a.ldx, k0, a.k, y);
+  if constexpr (OP == SILU) {
+    float u[8];
+    load8<T>(static_cast<const T*>(a.r) + row * a.ldr, k0, a.k, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = silu(y[i]) * u[i];
+  }
+  if constexpr (OP == NORM) {
+    float w[8];
+    load8<T>(static_cast<const T*>(a.w), k0, a.k, w);
+    if (a.r) {
+      float r[8];
+      load8<T>(static_cast<const T*>(a.r) + row * a.ldr, k0, a.k, r);
+      T h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        h[i] = from_f32<T>(y[i] + r[i]);
+        y[i] = to_f32<T>(h[i]);
+      }
+      if (write) store8<T>(static_cast<T*>(a.hidden) + row * a.ldh, k0, a.k, h);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ss = __builtin_fmaf(y[i], y[i], ss);
+      y[i] *= w[i];
+    }
+  }
+}
+
+// |y|'s bits: their integer order is the order of magnitudes, with NaN above infinity
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// 8 codes: rint(y * f) by the 1.5 * 2^23 shifter (|y * f| <= 127 up to an ulp), low bytes packed; `keep` 0 clears them
+__device__ __forceinline__ uint2 row_codes(const float (&y)[8], float pre, float f, uint32_t keep) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__builtin_fmaf(y[4 * h + i] * pre, f, MAGIC));
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    w[h] = (lo | hi) & keep;
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+template <int OP, typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_quant_kernel(RowArgs a) {
+  constexpr int WAVES = THREADS / 64, RPB = THREADS < 256 ? 256 / THREADS : 1;
+  static_assert(THREADS % 64 == 0, "whole waves per row");
+  const int t = threadIdx.x % THREADS;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / THREADS;
+  if (RPB > 1 && row >= a.m) return;  // (a whole wave leaves; such blocks have no barrier)
+  float y[NV ? NV : 1][8];
+  float ss = 0.0f;
+  uint32_t top = 0;
+  auto take = [&](const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[i]));
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int k0 = (j * THREADS + t) * 8;
+      if (k0 < a.k) {
+        row_values<OP, T>(a, row, k0, y[j], ss, true);
+        take(y[j]);
+      }
+    }
+  } else {
+    for (int64_t k0 = t * 8; k0 < a.k; k0 += THREADS * 8) {
+      row_values<OP, T>(a, row, (int)k0, y[0], ss, true);
+      take(y[0]);
+    }
+  }
+  // the wave's, then the row's, sum and maximum
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    if constexpr (OP == NORM) ss += __shfl_xor(ss, d);
+  }
+  if constexpr (WAVES > 1) {
+    __shared__ uint32_t tops[WAVES];
+    __shared__ float sums[WAVES];
+    if ((t & 63) == 0) {
+      tops[t >> 6] = top;
+      sums[t >> 6] = ss;
+    }
+    __syncthreads();
+    top = 0;
+    ss = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      top = max(top, tops[w]);
+      ss += sums[w];
+    }
+  }
+  float pre = 1.0f;
+  bool finite = top < 0x7f800000u;
+  if constexpr (OP == NORM) {
+    pre = 1.0f / sqrtf(ss / (float)a.k + a.eps);
+    finite = finite && abs_bits(ss) < 0x7f800000u;
+  }
+  const float m = fmaxf(__uint_as_float(top) * pre, ROW_TINY);
+  finite = finite && m < INFINITY;
+  const float f = 127.0f / m;
+  const uint32_t keep = finite ? 0xffffffffu : 0u;
+  if (t == 0) a.scales[row] = finite ? m / 127.0f : __uint_as_float(0x7fc00000u);
+  uint8_t* codes = reinterpret_cast<uint8_t*>(a.codes) + row * a.ldc;
+  auto put = [&](const float (&v)[8], int k0) {
+    const uint2 c = row_codes(v, pre, f, keep);
+    uint8_t b[8];
+    __builtin_memcpy(b, &c, 8);
+    store8<uint8_t>(codes, k0, a.k, b);
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int k0 = (j * THREADS + t) * 8;
+      if (k0 < a.k) put(y[j], k0);
+    }
+  } else {
+    for (int64_t k0 = t * 8; k0 < a.k; k0 += THREADS * 8) {
+      row_values<OP, T>(a, row, (int)k0, y[0], ss, false);
+      put(y[0], (int)k0);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ launches
+template <int OP, typename T, int THREADS, int NV>
+inline void launch_rows_form(const RowArgs& a, hipStream_t s) {
+  constexpr int RPB = THREADS < 256 ? 256 / THREADS : 1, BLOCK = THREADS * RPB;
+  // a grid dimension holds fewer than 2^32 threads: very many rows go in several launches
+  const int64_t most = ((int64_t)1 << 31) / BLOCK * RPB;
+  for (int64_t r0 = 0; r0 < a.m; r0 += most) {
+    RowArgs b = a;
+    b.m = a.m - r0 < most ? a.m - r0 : most;
+    b.x = static_cast<const T*>(a.x) + r0 * a.ldx;
+    if (a.r) b.r = static_cast<const T*>(a.r) + r0 * a.ldr;
+    b.codes = a.codes + r0 * a.ldc;
+    b.scales = a.scales + r0;
+    if (a.hidden) b.hidden = static_cast<T*>(a.hidden) + r0 * a.ldh;
+    row_quant_kernel<OP, T, THREADS, NV><<<dim3((unsigned)((b.m + RPB - 1) / RPB)), dim3(BLOCK), 0, s>>>(b);
+  }
+}
+
+// a wave per row while 4 vectors a lane hold it, then as many threads as do
+template <int OP, typename T>
+inline void launch_rows(const RowArgs& a, hipStream_t s) {
+  if (a.k <= 512) launch_rows_form<OP, T, 64, 1>(a, s);
+  else if (a.k <= 1024) launch_rows_form<OP, T, 64, 2>(a, s);
+  else if (a.k <= 2048) launch_rows_form<OP, T, 64, 4>(a, s);
+  else if (a.k <= 4096) launch_rows_form<OP, T, 256, 2>(a, s);
+  else if (a.k <= 8192) launch_rows_form<OP, T, 256, 4>(a, s);
+  else if (a.k <= 16384) launch_rows_form<OP, T, 512, 4>(a, s);
+  else if (a.k <= 24576) launch_rows_form<OP, T, 1024, 3>(a, s);
+  else if (a.k <= ROW_REGS) launch_rows_form<OP, T, 1024, 4>(a, s);
+  else launch_rows_form<OP, T, 1024, 0>(a, s);
+}
+template <int OP>
+inline void launch_rows(const RowArgs& a, int dtype, hipStream_t s) {
+  if (dtype == F32) launch_rows<OP, float>(a, s);
+  else if (dtype == BF16) launch_rows<OP, uint16_t>(a, s);
+  else launch_rows<OP, _Float16>(a, s);
+}
+
+}  // namespace tri

@@ -40,8 +40,10 @@ EXPORTS = ("tri_last_error", "tri_prepare_qk", "tri_pack_v", "tri_prepare", "tri
            "tri_decode", "tri_decode_partials", "tri_decode_merge", "tri_decode_short_tail",
            "tri_decode_merge_short_tail", "tri_decode_partials_timed", "tri_decode_noalloc",
            "tri_decode_tasks", "tri_cache_store", "tri_tail_spill", "tri_decode_occupancy", "tri_device_cus",
-           "tri_stream_read", "tri_issue_probe", "tri_prefill_pairs")
+           "tri_stream_read", "tri_issue_probe", "tri_prefill_pairs", "tri_quantize_rows", "tri_rms_norm_quant",
+           "tri_silu_mul_quant", "tri_int8_linear", "tri_int8_linear_workspace")
 KX_BYTES = 16384
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 TASK_WORDS = 512  # int32 words of the decode task table per (sequence, KV head, split)
 
 
@@ -86,6 +88,11 @@ def load_library() -> ctypes.CDLL:
     lib.tri_stream_read.argtypes = [P, I64, I, I, I, P, P]
     lib.tri_issue_probe.argtypes = [I, I, I, P, P]
     lib.tri_prefill_pairs.argtypes = [I]
+    lib.tri_quantize_rows.argtypes = [P, I64, I, I64, I64, P, I64, P, P]
+    lib.tri_rms_norm_quant.argtypes = [P, I64, P, I64, P, I, I64, I64, D_, P, I64, P, P, I64, P]
+    lib.tri_silu_mul_quant.argtypes = [P, I64, P, I64, I, I64, I64, P, I64, P, P]
+    lib.tri_int8_linear.argtypes = [P, I64, P, P, I64, P, P, P, I64, P, I64, I, I64, I64, I64, P, I64, P]
+    lib.tri_int8_linear_workspace.argtypes = [I64, I64, I64, ctypes.POINTER(ctypes.c_int64)]
     for name in EXPORTS:
         if name != "tri_last_error":
             getattr(lib, name).restype = ctypes.c_int
@@ -118,6 +125,7 @@ class Module:
     def __init__(self, lib: ctypes.CDLL):
         self.lib = lib
         self._plans = {}
+        self._workspaces = {}  # workspace bytes of the int8 products met so far, by shape
 
     def _call(self, fn, *args):
         if fn(*args) != 0:
@@ -534,6 +542,95 @@ class Module:
                 xb(dst["kx"]) if dst["xslot"] is not None else 0, p(table), int(n_tasks), 0]
         keep = (step, tail_base, ktail, vtail, grow, prompt, table, dict(dst))
         return SpillPlan(self, args, ktail.device, keep)
+
+    # ---------------------------------------------------------- 8-bit layer
+    @staticmethod
+    def _check_codes(x, codes, scales):
+        _check(codes.dtype == torch.int8 and codes.shape == x.shape and (codes.size(1) == 1 or codes.stride(1) == 1),
+               "codes int8 like the rows, with contiguous features")
+        _check(scales.dtype == torch.float32 and scales.is_contiguous() and scales.numel() == x.size(0), "scales fp32 [M]")
+        _check(codes.device == x.device and scales.device == x.device, "rows, codes and scales on one device")
+
+    @staticmethod
+    def _check_float_rows(x, what, like=None):
+        _check(x.dim() == 2 and x.dtype in _DTYPES and (x.size(1) == 1 or x.stride(1) == 1),
+               f"{what}: fp32, bf16 or fp16 rows [M,K] with contiguous features")
+        _check(like is None or (x.shape == like.shape and x.dtype == like.dtype and x.device == like.device),
+               f"{what}: of the other rows' shape, type and device")
+
+    def quantize_rows(self, x, codes, scales):
+        """int8 codes and one fp32 scale for each row of ``x`` [M,K] (tri_quantize_rows)."""
+        self._check_float_rows(x, "quantize_rows")
+        self._check_codes(x, codes, scales)
+        self._launch(x.device, self.lib.tri_quantize_rows, x.data_ptr(), x.stride(0), _DTYPES[x.dtype], x.size(0),
+                     x.size(1), codes.data_ptr(), codes.stride(0), scales.data_ptr())
+
+    def rms_norm_quant(self, x, residual, weight, eps, codes, scales, hidden):
+        """Codes and scales of ``rms_norm(x + residual) * weight``; ``hidden`` receives ``x + residual`` rounded to
+        x's type.  ``residual`` and ``hidden`` are both None or both rows like ``x`` (tri_rms_norm_quant)."""
+        self._check_float_rows(x, "rms_norm_quant")
+        self._check_codes(x, codes, scales)
+        _check(weight.dtype == x.dtype and weight.dim() == 1 and weight.numel() == x.size(1) and
+               weight.is_contiguous() and weight.device == x.device, "rms_norm_quant: weight [K] of x's type, on its device")
+        _check((residual is None) == (hidden is None), "rms_norm_quant: residual and hidden (both or neither)")
+        rows = (0, 0)
+        if residual is not None:
+            self._check_float_rows(residual, "rms_norm_quant: residual", x)
+            self._check_float_rows(hidden, "rms_norm_quant: hidden", x)
+            rows = residual.stride(0), hidden.stride(0)
+        self._launch(x.device, self.lib.tri_rms_norm_quant, x.data_ptr(), x.stride(0), _ptr(residual), rows[0],
+                     weight.data_ptr(), _DTYPES[x.dtype], x.size(0), x.size(1), float(eps), codes.data_ptr(),
+                     codes.stride(0), scales.data_ptr(), _ptr(hidden), rows[1])
+
+    def silu_mul_quant(self, gate, up, codes, scales):
+        """Codes and scales of ``silu(gate) * up`` (tri_silu_mul_quant)."""
+        self._check_float_rows(gate, "silu_mul_quant")
+        self._check_float_rows(up, "silu_mul_quant: up", gate)
+        self._check_codes(gate, codes, scales)
+        self._launch(gate.device, self.lib.tri_silu_mul_quant, gate.data_ptr(), gate.stride(0), up.data_ptr(),
+                     up.stride(0), _DTYPES[gate.dtype], gate.size(0), gate.size(1), codes.data_ptr(), codes.stride(0),
+                     scales.data_ptr())
+
+    def int8_linear_workspace(self, m, n, k, device) -> int:
+        """Bytes of workspace ``int8_linear`` needs for a product of [m,k] and [n,k] codes on ``device``."""
+        index = device.index if device.index is not None else torch.cuda.current_device()
+        found = self._workspaces.get((m, n, k, index))
+        if found is None:
+            size = ctypes.c_int64(0)
+            with torch.cuda.device(index):
+                self._call(self.lib.tri_int8_linear_workspace, m, n, k, ctypes.byref(size))
+            if len(self._workspaces) >= 4096:
+                self._workspaces.clear()
+            found = self._workspaces[(m, n, k, index)] = int(size.value)
+        return found
+
+    def int8_linear(self, x, xs, w, ws, bias, residual, out, workspace):
+        """``out = xs[:, None] * ws * (x @ w.T) + bias + residual`` of int8 codes ``x`` [M,K] and ``w`` [N,K]
+        (tri_int8_linear).  ``workspace``: uint8 of ``int8_linear_workspace`` bytes, None where that is 0."""
+        m, k = x.shape
+        n = w.size(0)
+        for codes, what in ((x, "x"), (w, "w")):
+            _check(codes.dtype == torch.int8 and codes.dim() == 2 and codes.size(1) == k and
+                   (k == 1 or codes.stride(1) == 1), f"int8_linear: {what} int8 codes [rows,K] with contiguous features")
+        _check(xs.dtype == ws.dtype == torch.float32 and xs.is_contiguous() and ws.is_contiguous() and
+               xs.numel() == m and ws.numel() == n, "int8_linear: scales fp32 [M] and [N]")
+        _check(out.dim() == 2 and tuple(out.shape) == (m, n) and out.dtype in _DTYPES and
+               (n == 1 or out.stride(1) == 1), "int8_linear: out fp32, bf16 or fp16 [M,N]")
+        _check(bias is None or (bias.dtype == out.dtype and bias.dim() == 1 and bias.numel() == n and
+                                bias.is_contiguous()), "int8_linear: bias [N] of out's type")
+        ldr = 0
+        if residual is not None:
+            _check(residual.dtype == out.dtype and residual.shape == out.shape and
+                   (n == 1 or residual.stride(1) == 1), "int8_linear: residual [M,N] of out's type")
+            ldr = residual.stride(0)
+        device = x.device
+        for t in (xs, w, ws, out, bias, residual, workspace):
+            _check(t is None or t.device == device, "int8_linear: operands on one device")
+        # (a single row's stride is never applied)
+        self._launch(device, self.lib.tri_int8_linear, x.data_ptr(), x.stride(0) if m > 1 else 0, xs.data_ptr(),
+                     w.data_ptr(), w.stride(0) if n > 1 else 0, ws.data_ptr(), _ptr(bias), _ptr(residual), ldr,
+                     out.data_ptr(), out.stride(0), _DTYPES[out.dtype], m, n, k, _ptr(workspace),
+                     0 if workspace is None else workspace.numel() * workspace.element_size())
 
     def decode_occupancy(self) -> int:
         """Resident decode workgroups per compute unit."""

@@ -1,0 +1,127 @@
+"""Host operators of the 8-bit layer around the quantized attention (no counterpart in the reference, whose
+projections, norms and activations run as the model's own bf16 modules).
+
+A W8A8 layer quantizes each token's hidden state to int8 with one scale, each output channel of a weight likewise,
+and multiplies the codes on the int8 matrix cores:
+
+    codes, scales, hidden = rms_norm_quant(x, norm.weight, eps, residual=hidden)
+    qkv = int8_linear(codes, scales, w_qkv, s_qkv, bias=b_qkv)
+    out = int8_linear(*quantize_rows(attention), w_o, s_o, residual=hidden)
+    down = int8_linear(*silu_mul_quant(gate, up), w_down, s_down)
+
+Weights are quantized by ``quantize_rows`` too (rows are output channels).  Every call allocates its outputs and, for
+products that are split over K, its own workspace, and runs on the current stream; all of them can be captured in a
+HIP graph.  Serving only: results carry no gradient, and a call on activations that ask for one is refused.
+
+Rows are the last dimension, features contiguous; the dimensions before it are free as long as the rows lie at one
+stride.  ``int8_linear`` takes codes whose rows start at multiples of 16 bytes, as the quantizers leave them.
+"""
+from __future__ import annotations
+
+import torch
+
+from .extension import load_extension
+
+
+def _rows(x, what):
+    """``x`` [..., K] as [M, K], without a copy."""
+    if x.dim() == 2:
+        return x
+    if x.dim() == 0:
+        raise RuntimeError(f"{what}: rows [..., K]")
+    if x.dim() == 1:
+        return x.unsqueeze(0)
+    try:
+        return x.view(x.shape[:-1].numel(), x.size(-1))
+    except RuntimeError:
+        raise RuntimeError(f"{what}: the rows of a {tuple(x.shape)} tensor with strides {x.stride()} do not lie at "
+                           f"one stride (pass x.contiguous())") from None
+
+
+def _serving(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient (call it under torch.no_grad() or inference_mode())")
+
+
+def _codes_like(x):
+    """Codes for rows [M, K], at a stride of a multiple of 16 bytes, and their scales."""
+    m, k = x.shape
+    pad = -k % 16
+    codes = torch.empty((m, k + pad), dtype=torch.int8, device=x.device)
+    return codes[:, :k] if pad else codes, torch.empty(m, dtype=torch.float32, device=x.device)
+
+
+def _shaped(x, codes, scales):
+    if x.dim() == 2:
+        return codes, scales
+    return codes.view(x.shape), scales.view(x.shape[:-1])
+
+
+def quantize_rows(x):
+    """(int8 codes like ``x``, fp32 scales of its rows): ``codes * scales[..., None]`` stands for ``x`` [..., K].
+
+    The scale is the row's largest magnitude / 127 and the code the nearest integer, half to even.  A row that holds an
+    infinity or a NaN gets scale NaN and codes 0.  x: fp32, bf16 or fp16."""
+    _serving("quantize_rows", x)
+    rows = _rows(x, "quantize_rows")
+    codes, scales = _codes_like(rows)
+    load_extension().quantize_rows(rows, codes, scales)
+    return _shaped(x, codes, scales)
+
+
+def rms_norm_quant(x, weight, eps, residual=None):
+    """(codes, scales, hidden) of the RMS norm of ``hidden = x + residual`` (``x`` itself without a residual).
+
+    hidden is rounded to x's type and the norm, ``hidden * rsqrt(mean(hidden^2) + eps) * weight``, is taken of it in
+    fp32 and quantized as ``quantize_rows`` does.  weight [K] of x's type; eps > 0."""
+    _serving("rms_norm_quant", x, residual)
+    rows = _rows(x, "rms_norm_quant")
+    codes, scales = _codes_like(rows)
+    hidden = x
+    other = out = None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise RuntimeError(f"rms_norm_quant: residual {tuple(residual.shape)} unlike x {tuple(x.shape)}")
+        other = _rows(residual, "rms_norm_quant: residual")
+        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _rows(hidden, "rms_norm_quant")
+    load_extension().rms_norm_quant(rows, other, weight, eps, codes, scales, out)
+    return *_shaped(x, codes, scales), hidden
+
+
+def silu_mul_quant(gate, up):
+    """(codes, scales) of ``silu(gate) * up`` in fp32, quantized as ``quantize_rows`` does.  gate and up may be the
+    halves of one fused projection's output."""
+    _serving("silu_mul_quant", gate, up)
+    if gate.shape != up.shape:
+        raise RuntimeError(f"silu_mul_quant: gate {tuple(gate.shape)} unlike up {tuple(up.shape)}")
+    rows = _rows(gate, "silu_mul_quant")
+    codes, scales = _codes_like(rows)
+    load_extension().silu_mul_quant(rows, _rows(up, "silu_mul_quant: up"), codes, scales)
+    return _shaped(gate, codes, scales)
+
+
+def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, out_dtype=torch.bfloat16):
+    """``scales[..., None] * weight_scales * (codes @ weight.T) + bias + residual`` as ``out_dtype``.
+
+    codes [..., K] int8 with scales [...] fp32, weight [N, K] int8 with weight_scales [N] fp32 (``quantize_rows`` of a
+    Linear's weight); bias [N] and residual [..., N] of ``out_dtype``.  The sums are exact int32, the rest fp32, rounded
+    once.  K from 1 to 131071; a row whose scale is NaN comes out NaN."""
+    _serving("int8_linear", scales, bias, residual)
+    x = _rows(codes, "int8_linear")
+    if scales.shape != codes.shape[:-1] or weight.dim() != 2 or weight.size(1) != x.size(1):
+        raise RuntimeError(f"int8_linear: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} and weight "
+                           f"{tuple(weight.shape)} do not go together ([..., K], [...], [N, K])")
+    m, n = x.size(0), weight.size(0)
+    shape = (*codes.shape[:-1], n)
+    other = None
+    if residual is not None:
+        if residual.shape != shape:
+            raise RuntimeError(f"int8_linear: residual {tuple(residual.shape)} unlike the output {shape}")
+        other = _rows(residual, "int8_linear: residual")
+    module = load_extension()
+    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    size = module.int8_linear_workspace(m, n, x.size(1), x.device) if m else 0
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    module.int8_linear(x, scales.reshape(m), weight, weight_scales, bias, other, out, workspace)
+    return out if codes.dim() == 2 else out.view(shape)
