@@ -1028,7 +1028,7 @@ int tri_silu_mul_quant(const void* gate, int64_t ldg, const void* up, int64_t ld
 static int linear_shape(int64_t m, int64_t n, int64_t k) {
   if (m < 0 || n < 1 || k < 1) return fail("int8_linear: empty shape");
   if (k > tri::LIN_MAX_K) return fail("int8_linear: at most %d input channels (int32 sums)", tri::LIN_MAX_K);
-  if (m > (1 << 30) || n > (1 << 30)) return fail("int8_linear: at most 2^30 rows and output channels");
+  if (m > (1 << 30) || n > (1 << 25)) return fail("int8_linear: at most 2^30 rows and 2^25 output channels");
   return 0;
 }
 
@@ -1058,6 +1058,7 @@ int tri_int8_linear(const int8_t* x, int64_t ldx, const float* xs, const int8_t*
   if (ldx < 0 || ldx > tri::LIN_MAX_LD || ldw < 0 || ldw > tri::LIN_MAX_LD)
     return fail("int8_linear: row strides of codes must be at most 4 MiB");
   if ((m > 1 && ldo < n) || (residual && ldr < 0)) return fail("int8_linear: row strides (output rows may not overlap)");
+  if (m > 1 && ldo > (1 << 25)) return fail("int8_linear: output row stride at most 2^25 elements");
   int cus = 0;
   if (device_cus(&cus)) return 1;
   const tri::LinearPlan p = tri::linear_plan((int)m, (int)n, (int)k, cus);
