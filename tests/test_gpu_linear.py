@@ -93,6 +93,26 @@ def test_silu_mul_quant(module, m, k, dtype):
     check_codes(codes, scales, gd * torch.sigmoid(gd) * up.double(), 127 * 16 * 2 * U, 16 * U)
 
 
+@pytest.mark.parametrize("m,k", [(4200, 4100), (1100, 18945), (33000, 511), (520, 33001)])
+def test_many_rows(module, m, k):
+    """Millions of elements, rows at odd strides, and the memory around the outputs left alone."""
+    g = gen(k)
+    wide = hidden(g, m, k + 3, torch.bfloat16)
+    x, w = wide[:, 1:1 + k], torch.ones(k, dtype=torch.bfloat16, device=DEV)
+    codes = torch.full((m + 2, k + 5), 99, dtype=torch.int8, device=DEV)
+    sums = torch.full((m + 2, k + 5), 7.0, dtype=torch.bfloat16, device=DEV)
+    scales = torch.full((m + 2,), 5.0, device=DEV)
+    module.rms_norm_quant(x, x, w, 1e-6, codes[1:-1, 2:2 + k], scales[1:-1], sums[1:-1, 2:2 + k])
+    h = (x.float() * 2).bfloat16()
+    assert torch.equal(sums[1:-1, 2:2 + k], h)
+    hd = h.double()
+    check_codes(codes[1:-1, 2:2 + k], scales[1:-1], hd / torch.sqrt(hd.square().mean(-1, keepdim=True) + 1e-6),
+                127 * 5 * U, (32 + 5) * U)
+    codes[1:-1, 2:2 + k], sums[1:-1, 2:2 + k], scales[1:-1] = 99, 7.0, 5.0
+    assert (codes == 99).all() and (sums == 7.0).all() and (scales == 5.0).all()
+    check_codes(*Q.quantize_rows(x), x.double(), 127 * 5 * U, 2 * U)
+
+
 def test_silu_of_far_negative_gates(module):
     # rows of negative gates alone: their own scale, down to where exp overflows (values of 0)
     gate = torch.stack([torch.linspace(-b, -b / 2, 300, device=DEV) for b in (1.0, 20.0, 60.0, 87.0, 300.0, 3e38)])

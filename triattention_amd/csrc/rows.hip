@@ -20,7 +20,6 @@ enum RowOp { ROWS = 0, NORM = 1, SILU = 2 };
 enum Dtype { F32 = 0, BF16 = 1, F16 = 2 };
 constexpr float ROW_TINY = 0x1p-118f;
 constexpr int ROW_REGS = 32768;  // longest row held in registers
-
 struct RowArgs {
   const void* x;         // x or gate
   const void* r;         // residual (may be null) or up
@@ -53,13 +52,27 @@ __device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return f32_to_
 template <>
 __device__ __forceinline__ _Float16 from_f32<_Float16>(float v) { return (_Float16)v; }
 
-// Elements k0 .. k0+7 of a row (0 past the row's end).  The vector access may be unaligned (rows of odd lengths or
-// strides): global memory takes it at the cost of split cache lines.
-template <typename T>
+// Rows are read and written past the caches (non-temporal): 8,191 x 4,096 norm with a residual 78 -> 45 us, 8,192 x
+// 18,944 SwiGLU 192 -> 132, 1,024 x 14,336 22 -> 17, 64 x 4,096 norm 7.3 -> 6.7; what is written is read next by workgroups of
+// all XCDs, which find little of it in their own L2.  The accesses may be unaligned (rows of odd lengths or strides):
+// global memory takes them at the cost of split cache lines.
+typedef v4i __attribute__((aligned(1))) v4i_any;
+typedef v2i __attribute__((aligned(1))) v2i_any;
+
+// Elements k0 .. k0+7 of a row (0 past the row's end); NT: past the caches.
+template <typename T, bool NT>
 __device__ __forceinline__ void load8(const T* __restrict__ row, int k0, int k, float (&v)[8]) {
   if (k0 + 8 <= k) {
     T t[8];
-    __builtin_memcpy(t, row + k0, sizeof(t));
+    if constexpr (NT) {
+      v4i q[sizeof(T) / 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        q[i] = __builtin_nontemporal_load(reinterpret_cast<const v4i_any*>(row + k0) + i);
+      __builtin_memcpy(t, q, sizeof(t));
+    } else {
+      __builtin_memcpy(t, row + k0, sizeof(t));
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
   } else {
@@ -69,12 +82,17 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int k0, int k, 
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* __restrict__ row, int k0, int k, const T (&t)[8]) {
-  if (k0 + 8 <= k) {
-    __builtin_memcpy(row + k0, t, sizeof(t));
-  } else {
+  if (k0 + 8 > k) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (k0 + i < k) row[k0 + i] = t[i];
+  } else if constexpr (sizeof(T) == 1) {
+    __builtin_memcpy(row + k0, t, 8);
+  } else {
+    v4i q[sizeof(T) / 2];
+    __builtin_memcpy(q, t, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_nontemporal_store(q[i], reinterpret_cast<v4i_any*>(row + k0) + i);
   }
 }
 
@@ -90,21 +108,21 @@ __device__ __forceinline__ float silu(float g) {
 }
 
 // y (NORM: h * w, still without the row's factor) of 8 elements; ss gathers h^2.
-template <int OP, typename T>
+template <int OP, typename T, bool NT>
 __device__ __forceinline__ void row_values(const RowArgs& a, int64_t row, int k0, float (&y)[8], float& ss, bool write) {
-  load8<T>(static_cast<const T*>(a.x) + row * a.ldx, k0, a.k, y);
+  load8<T, NT>(static_cast<const T*>(a.x) + row * a.ldx, k0, a.k, y);
   if constexpr (OP == SILU) {
     float u[8];
-    load8<T>(static_cast<const T*>(a.r) + row * a.ldr, k0, a.k, u);
+    load8<T, NT>(static_cast<const T*>(a.r) + row * a.ldr, k0, a.k, u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = silu(y[i]) * u[i];
   }
   if constexpr (OP == NORM) {
     float w[8];
-    load8<T>(static_cast<const T*>(a.w), k0, a.k, w);
+    load8<T, false>(static_cast<const T*>(a.w), k0, a.k, w);
     if (a.r) {
       float r[8];
-      load8<T>(static_cast<const T*>(a.r) + row * a.ldr, k0, a.k, r);
+      load8<T, NT>(static_cast<const T*>(a.r) + row * a.ldr, k0, a.k, r);
       T h[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -143,9 +161,10 @@ template <int OP, typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_quant_kernel(RowArgs a) {
   constexpr int WAVES = THREADS / 64, RPB = THREADS < 256 ? 256 / THREADS : 1;
   static_assert(THREADS % 64 == 0, "whole waves per row");
-  const int t = threadIdx.x % THREADS;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / THREADS;
-  if (RPB > 1 && row >= a.m) return;  // (a whole wave leaves; such blocks have no barrier)
+  const int t = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
+  const int64_t last = a.m - 1, row0 = (int64_t)blockIdx.x * RPB + sub;
+  const bool mine = RPB == 1 || row0 <= last;
+  const int64_t row = mine ? row0 : last;  // (a row past the last repeats it, for the barrier, and writes nothing)
   float y[NV ? NV : 1][8];
   float ss = 0.0f;
   uint32_t top = 0;
@@ -158,13 +177,13 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_quant_kerne
     for (int j = 0; j < NV; ++j) {
       const int k0 = (j * THREADS + t) * 8;
       if (k0 < a.k) {
-        row_values<OP, T>(a, row, k0, y[j], ss, true);
+        row_values<OP, T, true>(a, row, k0, y[j], ss, mine);
         take(y[j]);
       }
     }
   } else {
     for (int64_t k0 = t * 8; k0 < a.k; k0 += THREADS * 8) {
-      row_values<OP, T>(a, row, (int)k0, y[0], ss, true);
+      row_values<OP, T, false>(a, row, (int)k0, y[0], ss, mine);
       take(y[0]);
     }
   }
@@ -175,21 +194,22 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_quant_kerne
     if constexpr (OP == NORM) ss += __shfl_xor(ss, d);
   }
   if constexpr (WAVES > 1) {
-    __shared__ uint32_t tops[WAVES];
-    __shared__ float sums[WAVES];
+    __shared__ uint32_t tops[RPB][WAVES];
+    __shared__ float sums[RPB][WAVES];
     if ((t & 63) == 0) {
-      tops[t >> 6] = top;
-      sums[t >> 6] = ss;
+      tops[sub][t >> 6] = top;
+      sums[sub][t >> 6] = ss;
     }
     __syncthreads();
     top = 0;
     ss = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      top = max(top, tops[w]);
-      ss += sums[w];
+      top = max(top, tops[sub][w]);
+      ss += sums[sub][w];
     }
   }
+  if (!mine) return;
   float pre = 1.0f;
   bool finite = top < 0x7f800000u;
   if constexpr (OP == NORM) {
@@ -216,7 +236,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_quant_kerne
     }
   } else {
     for (int64_t k0 = t * 8; k0 < a.k; k0 += THREADS * 8) {
-      row_values<OP, T>(a, row, (int)k0, y[0], ss, false);
+      row_values<OP, T, false>(a, row, (int)k0, y[0], ss, false);
       put(y[0], (int)k0);
     }
   }
@@ -240,16 +260,17 @@ inline void launch_rows_form(const RowArgs& a, hipStream_t s) {
   }
 }
 
-// a wave per row while 4 vectors a lane hold it, then as many threads as do
+// The fewest threads that hold a row, two to five vectors each (more waves a row cost joins, more vectors a thread
+// occupancy: 18,944 columns as 512 x 5 132 us, 1,024 x 3 145; 4,096 as 256 x 2 45, 512 x 1 48).
 template <int OP, typename T>
 inline void launch_rows(const RowArgs& a, hipStream_t s) {
   if (a.k <= 512) launch_rows_form<OP, T, 64, 1>(a, s);
   else if (a.k <= 1024) launch_rows_form<OP, T, 64, 2>(a, s);
-  else if (a.k <= 2048) launch_rows_form<OP, T, 64, 4>(a, s);
+  else if (a.k <= 2048) launch_rows_form<OP, T, 128, 2>(a, s);
   else if (a.k <= 4096) launch_rows_form<OP, T, 256, 2>(a, s);
-  else if (a.k <= 8192) launch_rows_form<OP, T, 256, 4>(a, s);
+  else if (a.k <= 8192) launch_rows_form<OP, T, 512, 2>(a, s);
   else if (a.k <= 16384) launch_rows_form<OP, T, 512, 4>(a, s);
-  else if (a.k <= 24576) launch_rows_form<OP, T, 1024, 3>(a, s);
+  else if (a.k <= 20480) launch_rows_form<OP, T, 512, 5>(a, s);
   else if (a.k <= ROW_REGS) launch_rows_form<OP, T, 1024, 4>(a, s);
   else launch_rows_form<OP, T, 1024, 0>(a, s);
 }

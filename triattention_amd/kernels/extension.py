@@ -544,51 +544,67 @@ class Module:
         return SpillPlan(self, args, ktail.device, keep)
 
     # ---------------------------------------------------------- 8-bit layer
+    # (each op checks its operands, then its outputs; the host operators, which allocate the outputs, skip the second)
+    @staticmethod
+    def _check_float_rows(x, what, like=None):
+        if x.dim() != 2 or x.dtype not in _DTYPES or (x.stride(1) != 1 and x.size(1) != 1):
+            raise RuntimeError(f"{what}: fp32, bf16 or fp16 rows [M,K] with contiguous features")
+        if like is not None and (x.shape != like.shape or x.dtype != like.dtype or x.device != like.device):
+            raise RuntimeError(f"{what}: not of the other rows' shape, type and device")
+
     @staticmethod
     def _check_codes(x, codes, scales):
-        _check(codes.dtype == torch.int8 and codes.shape == x.shape and (codes.size(1) == 1 or codes.stride(1) == 1),
+        _check(codes.dtype == torch.int8 and codes.shape == x.shape and (codes.stride(1) == 1 or codes.size(1) == 1),
                "codes int8 like the rows, with contiguous features")
         _check(scales.dtype == torch.float32 and scales.is_contiguous() and scales.numel() == x.size(0), "scales fp32 [M]")
         _check(codes.device == x.device and scales.device == x.device, "rows, codes and scales on one device")
-
-    @staticmethod
-    def _check_float_rows(x, what, like=None):
-        _check(x.dim() == 2 and x.dtype in _DTYPES and (x.size(1) == 1 or x.stride(1) == 1),
-               f"{what}: fp32, bf16 or fp16 rows [M,K] with contiguous features")
-        _check(like is None or (x.shape == like.shape and x.dtype == like.dtype and x.device == like.device),
-               f"{what}: of the other rows' shape, type and device")
 
     def quantize_rows(self, x, codes, scales):
         """int8 codes and one fp32 scale for each row of ``x`` [M,K] (tri_quantize_rows)."""
         self._check_float_rows(x, "quantize_rows")
         self._check_codes(x, codes, scales)
+        self._quantize_rows(x, codes, codes.stride(0), scales)
+
+    def _quantize_rows(self, x, codes, ldc, scales):
         self._launch(x.device, self.lib.tri_quantize_rows, x.data_ptr(), x.stride(0), _DTYPES[x.dtype], x.size(0),
-                     x.size(1), codes.data_ptr(), codes.stride(0), scales.data_ptr())
+                     x.size(1), codes.data_ptr(), ldc, scales.data_ptr())
+
+    def _check_norm(self, x, residual, weight):
+        self._check_float_rows(x, "rms_norm_quant")
+        _check(weight.dtype == x.dtype and weight.dim() == 1 and weight.numel() == x.size(1) and
+               weight.is_contiguous() and weight.device == x.device, "rms_norm_quant: weight [K] of x's type, on its device")
+        if residual is not None:
+            self._check_float_rows(residual, "rms_norm_quant: residual", x)
 
     def rms_norm_quant(self, x, residual, weight, eps, codes, scales, hidden):
         """Codes and scales of ``rms_norm(x + residual) * weight``; ``hidden`` receives ``x + residual`` rounded to
         x's type.  ``residual`` and ``hidden`` are both None or both rows like ``x`` (tri_rms_norm_quant)."""
-        self._check_float_rows(x, "rms_norm_quant")
+        self._check_norm(x, residual, weight)
         self._check_codes(x, codes, scales)
-        _check(weight.dtype == x.dtype and weight.dim() == 1 and weight.numel() == x.size(1) and
-               weight.is_contiguous() and weight.device == x.device, "rms_norm_quant: weight [K] of x's type, on its device")
         _check((residual is None) == (hidden is None), "rms_norm_quant: residual and hidden (both or neither)")
-        rows = (0, 0)
-        if residual is not None:
-            self._check_float_rows(residual, "rms_norm_quant: residual", x)
+        if hidden is not None:
             self._check_float_rows(hidden, "rms_norm_quant: hidden", x)
-            rows = residual.stride(0), hidden.stride(0)
-        self._launch(x.device, self.lib.tri_rms_norm_quant, x.data_ptr(), x.stride(0), _ptr(residual), rows[0],
-                     weight.data_ptr(), _DTYPES[x.dtype], x.size(0), x.size(1), float(eps), codes.data_ptr(),
-                     codes.stride(0), scales.data_ptr(), _ptr(hidden), rows[1])
+        self._rms_norm_quant(x, residual, weight, eps, codes, codes.stride(0), scales, hidden,
+                             0 if hidden is None else hidden.stride(0))
+
+    def _rms_norm_quant(self, x, residual, weight, eps, codes, ldc, scales, hidden, ldh):
+        self._launch(x.device, self.lib.tri_rms_norm_quant, x.data_ptr(), x.stride(0), _ptr(residual),
+                     0 if residual is None else residual.stride(0), weight.data_ptr(), _DTYPES[x.dtype], x.size(0),
+                     x.size(1), eps, codes.data_ptr(), ldc, scales.data_ptr(), _ptr(hidden), ldh)
+
+    def _check_silu(self, gate, up):
+        self._check_float_rows(gate, "silu_mul_quant")
+        self._check_float_rows(up, "silu_mul_quant: up", gate)
 
     def silu_mul_quant(self, gate, up, codes, scales):
         """Codes and scales of ``silu(gate) * up`` (tri_silu_mul_quant)."""
-        self._check_float_rows(gate, "silu_mul_quant")
-        self._check_float_rows(up, "silu_mul_quant: up", gate)
+        self._check_silu(gate, up)
         self._check_codes(gate, codes, scales)
+        self._silu_mul_quant(gate, up, codes, codes.stride(0), scales)
+
+    def _silu_mul_quant(self, gate, up, codes, ldc, scales):
         self._launch(gate.device, self.lib.tri_silu_mul_quant, gate.data_ptr(), gate.stride(0), up.data_ptr(),
-                     up.stride(0), _DTYPES[gate.dtype], gate.size(0), gate.size(1), codes.data_ptr(), codes.stride(0),
+                     up.stride(0), _DTYPES[gate.dtype], gate.size(0), gate.size(1), codes.data_ptr(), ldc,
                      scales.data_ptr())
 
     def int8_linear_workspace(self, m, n, k, device) -> int:
@@ -604,33 +620,44 @@ class Module:
             found = self._workspaces[(m, n, k, index)] = int(size.value)
         return found
 
+    @staticmethod
+    def _check_linear(x, xs, w, ws, bias, residual, dtype):
+        k, device = x.size(1), x.device
+        _check(x.dtype == w.dtype == torch.int8 and w.dim() == 2 and w.size(1) == k and w.device == device and
+               (k == 1 or (x.stride(1) == 1 and w.stride(1) == 1)),
+               "int8_linear: int8 codes [M,K] and [N,K] with contiguous features, on one device")
+        n = w.size(0)
+        _check(xs.dtype == ws.dtype == torch.float32 and xs.numel() == x.size(0) and ws.numel() == n and
+               xs.is_contiguous() and ws.is_contiguous() and xs.device == device and ws.device == device,
+               "int8_linear: scales fp32 [M] and [N], contiguous, on the codes' device")
+        _check(dtype in _DTYPES, "int8_linear: out fp32, bf16 or fp16")
+        _check(bias is None or (bias.dtype == dtype and bias.dim() == 1 and bias.numel() == n and
+                                bias.is_contiguous() and bias.device == device),
+               "int8_linear: bias [N] of out's type, on the codes' device")
+        _check(residual is None or (residual.dtype == dtype and residual.dim() == 2 and
+                                    residual.size(0) == x.size(0) and residual.size(1) == n and
+                                    (residual.stride(1) == 1 or n == 1) and residual.device == device),
+               "int8_linear: residual [M,N] of out's type, with contiguous features, on the codes' device")
+
     def int8_linear(self, x, xs, w, ws, bias, residual, out, workspace):
         """``out = xs[:, None] * ws * (x @ w.T) + bias + residual`` of int8 codes ``x`` [M,K] and ``w`` [N,K]
         (tri_int8_linear).  ``workspace``: uint8 of ``int8_linear_workspace`` bytes, None where that is 0."""
-        m, k = x.shape
-        n = w.size(0)
-        for codes, what in ((x, "x"), (w, "w")):
-            _check(codes.dtype == torch.int8 and codes.dim() == 2 and codes.size(1) == k and
-                   (k == 1 or codes.stride(1) == 1), f"int8_linear: {what} int8 codes [rows,K] with contiguous features")
-        _check(xs.dtype == ws.dtype == torch.float32 and xs.is_contiguous() and ws.is_contiguous() and
-               xs.numel() == m and ws.numel() == n, "int8_linear: scales fp32 [M] and [N]")
-        _check(out.dim() == 2 and tuple(out.shape) == (m, n) and out.dtype in _DTYPES and
-               (n == 1 or out.stride(1) == 1), "int8_linear: out fp32, bf16 or fp16 [M,N]")
-        _check(bias is None or (bias.dtype == out.dtype and bias.dim() == 1 and bias.numel() == n and
-                                bias.is_contiguous()), "int8_linear: bias [N] of out's type")
-        ldr = 0
-        if residual is not None:
-            _check(residual.dtype == out.dtype and residual.shape == out.shape and
-                   (n == 1 or residual.stride(1) == 1), "int8_linear: residual [M,N] of out's type")
-            ldr = residual.stride(0)
-        device = x.device
-        for t in (xs, w, ws, out, bias, residual, workspace):
-            _check(t is None or t.device == device, "int8_linear: operands on one device")
+        _check(x.dim() == 2, "int8_linear: int8 codes [M,K]")
+        self._check_linear(x, xs, w, ws, bias, residual, out.dtype)
+        _check(out.dim() == 2 and out.size(0) == x.size(0) and out.size(1) == w.size(0) and
+               (out.size(1) == 1 or out.stride(1) == 1) and out.device == x.device,
+               "int8_linear: out [M,N] with contiguous features, on the codes' device")
+        _check(workspace is None or (workspace.is_contiguous() and workspace.device == x.device),
+               "int8_linear: workspace on the codes' device")
+        self._int8_linear(x, xs, w, ws, bias, residual, out, out.stride(0), workspace)
+
+    def _int8_linear(self, x, xs, w, ws, bias, residual, out, ldo, workspace):
+        m, n = x.size(0), w.size(0)
         # (a single row's stride is never applied)
-        self._launch(device, self.lib.tri_int8_linear, x.data_ptr(), x.stride(0) if m > 1 else 0, xs.data_ptr(),
-                     w.data_ptr(), w.stride(0) if n > 1 else 0, ws.data_ptr(), _ptr(bias), _ptr(residual), ldr,
-                     out.data_ptr(), out.stride(0), _DTYPES[out.dtype], m, n, k, _ptr(workspace),
-                     0 if workspace is None else workspace.numel() * workspace.element_size())
+        self._launch(x.device, self.lib.tri_int8_linear, x.data_ptr(), x.stride(0) if m > 1 else 0, xs.data_ptr(),
+                     w.data_ptr(), w.stride(0) if n > 1 else 0, ws.data_ptr(), _ptr(bias), _ptr(residual),
+                     0 if residual is None else residual.stride(0), out.data_ptr(), ldo, _DTYPES[out.dtype], m, n,
+                     x.size(1), _ptr(workspace), 0 if workspace is None else workspace.nbytes)
 
     def decode_occupancy(self) -> int:
         """Resident decode workgroups per compute unit."""

@@ -43,18 +43,13 @@ def _serving(what, *tensors):
         raise RuntimeError(f"{what} has no gradient (call it under torch.no_grad() or inference_mode())")
 
 
-def _codes_like(x):
-    """Codes for rows [M, K], at a stride of a multiple of 16 bytes, and their scales."""
-    m, k = x.shape
-    pad = -k % 16
-    codes = torch.empty((m, k + pad), dtype=torch.int8, device=x.device)
-    return codes[:, :k] if pad else codes, torch.empty(m, dtype=torch.float32, device=x.device)
-
-
-def _shaped(x, codes, scales):
-    if x.dim() == 2:
-        return codes, scales
-    return codes.view(x.shape), scales.view(x.shape[:-1])
+def _outputs(x):
+    """Codes like ``x`` [..., K] at a row stride of a multiple of 16 bytes, the stride, and the rows' scales."""
+    k = x.size(-1)
+    ld = k + -k % 16
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    codes = torch.empty((*x.shape[:-1], ld), dtype=torch.int8, device=x.device)
+    return codes if ld == k else codes[..., :k], ld, scales
 
 
 def quantize_rows(x):
@@ -62,11 +57,13 @@ def quantize_rows(x):
 
     The scale is the row's largest magnitude / 127 and the code the nearest integer, half to even.  A row that holds an
     infinity or a NaN gets scale NaN and codes 0.  x: fp32, bf16 or fp16."""
-    _serving("quantize_rows", x)
-    rows = _rows(x, "quantize_rows")
-    codes, scales = _codes_like(rows)
-    load_extension().quantize_rows(rows, codes, scales)
-    return _shaped(x, codes, scales)
+    if x.requires_grad:
+        _serving("quantize_rows", x)
+    module, rows = load_extension(), _rows(x, "quantize_rows")
+    module._check_float_rows(rows, "quantize_rows")
+    codes, ld, scales = _outputs(x)
+    module._quantize_rows(rows, codes, ld, scales)
+    return codes, scales
 
 
 def rms_norm_quant(x, weight, eps, residual=None):
@@ -74,31 +71,35 @@ def rms_norm_quant(x, weight, eps, residual=None):
 
     hidden is rounded to x's type and the norm, ``hidden * rsqrt(mean(hidden^2) + eps) * weight``, is taken of it in
     fp32 and quantized as ``quantize_rows`` does.  weight [K] of x's type; eps > 0."""
-    _serving("rms_norm_quant", x, residual)
-    rows = _rows(x, "rms_norm_quant")
-    codes, scales = _codes_like(rows)
-    hidden = x
-    other = out = None
+    if x.requires_grad or (residual is not None and residual.requires_grad):
+        _serving("rms_norm_quant", x, residual)
+    module, rows = load_extension(), _rows(x, "rms_norm_quant")
+    hidden, other, sums = x, None, None
     if residual is not None:
         if residual.shape != x.shape:
             raise RuntimeError(f"rms_norm_quant: residual {tuple(residual.shape)} unlike x {tuple(x.shape)}")
         other = _rows(residual, "rms_norm_quant: residual")
-        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        out = _rows(hidden, "rms_norm_quant")
-    load_extension().rms_norm_quant(rows, other, weight, eps, codes, scales, out)
-    return *_shaped(x, codes, scales), hidden
+    module._check_norm(rows, other, weight)
+    codes, ld, scales = _outputs(x)
+    if residual is not None:
+        hidden = sums = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    module._rms_norm_quant(rows, other, weight, eps, codes, ld, scales, sums, x.size(-1))
+    return codes, scales, hidden
 
 
 def silu_mul_quant(gate, up):
     """(codes, scales) of ``silu(gate) * up`` in fp32, quantized as ``quantize_rows`` does.  gate and up may be the
     halves of one fused projection's output."""
-    _serving("silu_mul_quant", gate, up)
+    if gate.requires_grad or up.requires_grad:
+        _serving("silu_mul_quant", gate, up)
     if gate.shape != up.shape:
         raise RuntimeError(f"silu_mul_quant: gate {tuple(gate.shape)} unlike up {tuple(up.shape)}")
-    rows = _rows(gate, "silu_mul_quant")
-    codes, scales = _codes_like(rows)
-    load_extension().silu_mul_quant(rows, _rows(up, "silu_mul_quant: up"), codes, scales)
-    return _shaped(gate, codes, scales)
+    module = load_extension()
+    rows, other = _rows(gate, "silu_mul_quant"), _rows(up, "silu_mul_quant: up")
+    module._check_silu(rows, other)
+    codes, ld, scales = _outputs(gate)
+    module._silu_mul_quant(rows, other, codes, ld, scales)
+    return codes, scales
 
 
 def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, out_dtype=torch.bfloat16):
@@ -107,7 +108,9 @@ def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, 
     codes [..., K] int8 with scales [...] fp32, weight [N, K] int8 with weight_scales [N] fp32 (``quantize_rows`` of a
     Linear's weight); bias [N] and residual [..., N] of ``out_dtype``.  The sums are exact int32, the rest fp32, rounded
     once.  K from 1 to 131071; a row whose scale is NaN comes out NaN."""
-    _serving("int8_linear", scales, bias, residual)
+    if scales.requires_grad or (bias is not None and bias.requires_grad) or \
+            (residual is not None and residual.requires_grad):
+        _serving("int8_linear", scales, bias, residual)
     x = _rows(codes, "int8_linear")
     if scales.shape != codes.shape[:-1] or weight.dim() != 2 or weight.size(1) != x.size(1):
         raise RuntimeError(f"int8_linear: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} and weight "
@@ -120,8 +123,9 @@ def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, 
             raise RuntimeError(f"int8_linear: residual {tuple(residual.shape)} unlike the output {shape}")
         other = _rows(residual, "int8_linear: residual")
     module = load_extension()
-    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    module._check_linear(x, scales, weight, weight_scales, bias, other, out_dtype)
+    out = torch.empty(shape, dtype=out_dtype, device=x.device)
     size = module.int8_linear_workspace(m, n, x.size(1), x.device) if m else 0
     workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    module.int8_linear(x, scales.reshape(m), weight, weight_scales, bias, other, out, workspace)
-    return out if codes.dim() == 2 else out.view(shape)
+    module._int8_linear(x, scales, weight, weight_scales, bias, other, out, n, workspace)
+    return out
