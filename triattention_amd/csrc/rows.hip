@@ -52,12 +52,12 @@ __device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return f32_to_
 template <>
 __device__ __forceinline__ _Float16 from_f32<_Float16>(float v) { return (_Float16)v; }
 
-// Rows are read and written past the caches (non-temporal): 8,191 x 4,096 norm with a residual 78 -> 45 us, 8,192 x
-// 18,944 SwiGLU 192 -> 132, 1,024 x 14,336 22 -> 17, 64 x 4,096 norm 7.3 -> 6.7; what is written is read next by workgroups of
-// all XCDs, which find little of it in their own L2.  The accesses may be unaligned (rows of odd lengths or strides):
-// global memory takes them at the cost of split cache lines.
+// Rows are read past the caches (non-temporal loads) and the sums of NORM written so: 8,191 x 4,096 norm with a residual
+// 78 -> 54 us with the loads, 48 with both; 8,192 x 18,944 SwiGLU 192 -> 131; 1,024 x 14,336 22 -> 17; 64 x 4,096 norm 7.3
+// -> 6.7.  Codes, a third of the bytes, are written the ordinary way: that costs nothing here and the product that reads
+// them next finds them nearer (a copy of 68 MB of them 185 -> 154 us).  The accesses may be unaligned (rows of odd lengths or
+// strides): global memory takes them at the cost of split cache lines.
 typedef v4i __attribute__((aligned(1))) v4i_any;
-typedef v2i __attribute__((aligned(1))) v2i_any;
 
 // Elements k0 .. k0+7 of a row (0 past the row's end); NT: past the caches.
 template <typename T, bool NT>

@@ -129,3 +129,39 @@ def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, 
     workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     module._int8_linear(x, scales, weight, weight_scales, bias, other, out, n, workspace)
     return out
+
+
+class Int8Linear(torch.nn.Module):
+    """One or more Linears over the same input as one int8 product: the rows of their weights as codes and scales, one
+    after another, and their biases.
+
+    ``layer(x)`` quantizes the rows of ``x``; ``layer(codes, scales)`` takes them as they are.  The output has the type
+    of the Linears' weights; ``residual`` is added in it."""
+
+    def __init__(self, *linears):
+        super().__init__()
+        first = linears[0].weight
+        if any(l.weight.dtype != first.dtype or l.weight.size(1) != first.size(1) for l in linears):
+            raise ValueError("Int8Linear: Linears of one type over one input width")
+        with torch.no_grad():
+            n, k = sum(l.weight.size(0) for l in linears), first.size(1)
+            codes = torch.empty((n, k + -k % 16), dtype=torch.int8, device=first.device)[:, :k]
+            scales = torch.empty(n, dtype=torch.float32, device=first.device)
+            bias, at = None, 0
+            if any(l.bias is not None for l in linears):
+                bias = torch.zeros(n, dtype=first.dtype, device=first.device)
+            for l in linears:
+                end = at + l.weight.size(0)
+                codes[at:end], scales[at:end] = quantize_rows(l.weight.detach())
+                if l.bias is not None:
+                    bias[at:end] = l.bias
+                at = end
+        self.dtype = first.dtype
+        self.register_buffer("codes", codes)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", bias)
+
+    def forward(self, x, scales=None, residual=None):
+        if scales is None:
+            x, scales = quantize_rows(x)
+        return int8_linear(x, scales, self.codes, self.scales, self.bias, residual, self.dtype)

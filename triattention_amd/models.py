@@ -34,10 +34,12 @@ be handed to ``TriAttention``, however it was loaded.
 from __future__ import annotations
 
 import os
+import types
 
 import torch
 
 from .kernels.decode import DecodeCache
+from .kernels import linear
 from .kernels.extension import load_extension
 from .kernels.prefill import Prefill
 from .maps import INF, load_map, preset
@@ -146,6 +148,86 @@ def use_attention(model, name, fn):
 
     ALL_ATTENTION_FUNCTIONS[name] = attention
     model.set_attn_implementation(name)
+
+
+class _Codes:
+    """Hidden states as int8 codes and scales, in a tensor's place as a layer's attention takes them; ``parts`` holds
+    the fused projections' output once the first of them has run."""
+
+    def __init__(self, codes, scales):
+        self.codes, self.scales, self.shape, self.parts = codes, scales, codes.shape, None
+
+
+class _Part(torch.nn.Module):
+    """One of the Q, K and V projections: its slice of their one product."""
+
+    def __init__(self, fused, index, sizes):
+        super().__init__()
+        self.fused, self.index, self.sizes = fused, index, sizes
+
+    def forward(self, x):
+        if not isinstance(x, _Codes):
+            x = _Codes(*linear.quantize_rows(x))
+        if x.parts is None:
+            x.parts = self.fused(x.codes, x.scales).split(self.sizes, -1)
+        # (dense, as a Linear of its own leaves it: the decode cache takes K and V at the same strides)
+        return x.parts[self.index].contiguous()
+
+
+def _int8_layer_forward(self, hidden_states, **kwargs):
+    """A decoder layer's forward on int8 products: the norms quantize what the projections read, the residual goes
+    through the second norm's sum and the down projection's epilogue."""
+    first, second = self.input_layernorm, self.post_attention_layernorm
+    codes, scales, _ = linear.rms_norm_quant(hidden_states, first.weight, first.variance_epsilon)
+    attended, _ = self.self_attn(hidden_states=_Codes(codes, scales), **kwargs)
+    codes, scales, hidden = linear.rms_norm_quant(attended, second.weight, second.variance_epsilon,
+                                                  residual=hidden_states)
+    gate, up = self.mlp.gate_up(codes, scales).chunk(2, -1)
+    return self.mlp.down(*linear.silu_mul_quant(gate, up), residual=hidden)
+
+
+_INT8_LAYERS = ("LlamaDecoderLayer", "MistralDecoderLayer", "Ministral3DecoderLayer", "Qwen2DecoderLayer")
+
+
+def use_int8_layers(model, lm_head=False):
+    """Run the projections, norms and SwiGLU of ``model``'s decoder layers in 8 bits (extension): int8 codes with a
+    scale for each token and each output channel, in place, for inference.  The attention stays what the model is set
+    to (``TriAttention``, ``use_attention``), and so do embeddings, the last norm and, without ``lm_head``, the head.
+
+    Takes the layers of Llama, Qwen2, Mistral and Ministral 3 checkpoints, with SwiGLU; a model with none of them is
+    refused, unchanged.  Their floating weights are dropped.  Returns the number of layers converted."""
+    layers = [m for m in model.modules() if type(m).__name__ in _INT8_LAYERS]
+    if not layers:
+        raise ValueError(f"no decoder layer of a kind that runs in 8 bits ({', '.join(_INT8_LAYERS)})")
+    if model.training:
+        raise ValueError("8-bit layers are for inference: call model.eval() first")
+    head = model.get_output_embeddings() if lm_head else None
+    for layer in layers:
+        attention, mlp = layer.self_attn, layer.mlp
+        if isinstance(attention.q_proj, _Part):
+            raise ValueError("the model's layers run in 8 bits already")
+        if not isinstance(mlp.act_fn, torch.nn.SiLU) and type(mlp.act_fn).__name__ not in ("SiLU", "SiLUActivation"):
+            raise ValueError(f"8-bit layers need SwiGLU, not {type(mlp.act_fn).__name__}")
+        for l in (attention.q_proj, attention.k_proj, attention.v_proj, attention.o_proj, mlp.gate_proj, mlp.up_proj,
+                  mlp.down_proj) + ((head,) if lm_head else ()):
+            if type(l) is not torch.nn.Linear:
+                raise ValueError(f"8-bit layers are made from torch.nn.Linear, not {type(l).__name__}")
+        if mlp.gate_proj.out_features != mlp.up_proj.out_features:
+            raise ValueError("gate and up projections of different widths")
+    for layer in layers:
+        attention, mlp = layer.self_attn, layer.mlp
+        projections = (attention.q_proj, attention.k_proj, attention.v_proj)
+        sizes = [l.out_features for l in projections]
+        fused = linear.Int8Linear(*projections)
+        attention.q_proj, attention.k_proj, attention.v_proj = (_Part(fused, i, sizes) for i in range(3))
+        attention.o_proj = linear.Int8Linear(attention.o_proj)
+        layer.mlp = torch.nn.Module()
+        layer.mlp.gate_up = linear.Int8Linear(mlp.gate_proj, mlp.up_proj)
+        layer.mlp.down = linear.Int8Linear(mlp.down_proj)
+        layer.forward = types.MethodType(_int8_layer_forward, layer)
+    if lm_head:
+        model.set_output_embeddings(linear.Int8Linear(head))
+    return len(layers)
 
 
 class TriAttention:
