@@ -2,16 +2,20 @@
 // x [M][K] and w [N][K] int8 rows, int32 sums (exact: K <= 131071 keeps 128 * 128 * K below 2^31), the epilogue in fp32,
 // one rounding to the output's type.
 //
-// dot_kernel: up to DOT_M rows of x.  The work is the stream of w: a wave reads 8 rows x 128 bytes per
-// load (8 lanes a row, whole cache lines), takes v_dot4_i32_i8 against the rows of x, and the waves of a workgroup
-// share the K axis.  16 rows x 64 bytes, the MFMA's own operand order, reads at 0.7 of that rate.
+// dot_kernel, up to 4 rows of x: the work is the stream of w.  A wave reads 8 rows x 128 bytes per load (8 lanes a row,
+// whole cache lines), takes v_dot4_i32_i8 against the rows of x, and the waves of a workgroup share the K axis.  (16 rows x
+// 64 bytes, the MFMA's own operand order, streams at 0.7 of that rate.)  1 row x 152,064 channels x 3,584: 77 us, 7.0 TB/s;
+// x 3,584 x 18,944: 11.8 us, 5.8 TB/s.
 //
-// tile_kernel: BM x BN outputs per workgroup.  Both operands go to LDS 128 bytes of K at a time by
-// direct loads (8 rows x 128 bytes per wave and load), in two buffers: the loads of step s + 1 are in flight while the
-// MFMAs of step s run.  16-byte chunk c of row r sits at slot c ^ (r & 7), so that the MFMA operand reads (one chunk
-// of 16 or 32 rows) touch every bank once per phase.  w is the MFMA's first operand: a lane then holds four
-// consecutive n of one m.  Rows past M or N read the last row, chunks past K the row's last chunk; what they add is
-// masked (K, on x) or not stored (M, N).
+// tile_kernel, BM x BN outputs per workgroup: both operands go to LDS 128 bytes of K a step by direct loads (8 rows x 128
+// bytes per wave and load) into two to four buffers, awaited by count, so that one to three steps are in flight.
+// 16-byte chunk c of row r sits at slot c ^ (r & 7), so that the MFMA operand reads (one chunk of 16 or 32 rows) touch
+// every bank once per phase.  Loads and reads are spread among the MFMAs.  w is the MFMA's first operand: a lane then
+// holds four consecutive n of one m.  Rows past M or N read the last row, chunks past K the row's last chunk; what they
+// add is masked (K, on x) or not stored (M, N).  The largest form, 256 x 256 by four waves of 128 x 128, is bound by the
+// card's power: its clock falls to 1.6-2.0 GHz (2.4 idle), a step takes 2,600-2,800 cycles of 2,048 MFMA cycles; eight waves
+// of 128 x 64 take fewer cycles, read half as much LDS again and, at 1.4-1.75 GHz, more time.  8,192 x 37,888 x 3,584: 1,042 us
+// (2,130 Top/s; the library's int8 product 1,146), 8,192^3 450 us (2,440 Top/s; 545).
 //
 // With few tiles the K axis is split over workgroups: int32 partials, summed by linear_join_kernel.
 #pragma once
@@ -49,12 +53,25 @@ __device__ __forceinline__ float lin_f32(T v) { return (float)v; }
 template <>
 __device__ __forceinline__ float lin_f32<__bf16>(__bf16 v) { return bf16f(__builtin_bit_cast(uint16_t, v)); }
 
-// `run` with a value of the output's type
-template <typename F>
-__device__ __forceinline__ void lin_typed(int dtype, F run) {
-  if (dtype == BF16) run(__bf16{});
-  else if (dtype == F32) run(float{});
-  else run(_Float16{});
+// What of a tile exists: all of it, every channel of the rows that do, or less.
+enum LinearPart { LIN_EDGE = 0, LIN_ROWS = 1, LIN_WHOLE = 2 };
+template <int P>
+using lin_part = std::integral_constant<int, P>;
+// run(a value of the output's type, the part, whether there is a residual), each as a constant
+template <bool WHOLE = true, typename F>
+__device__ __forceinline__ void lin_typed(const LinearArgs& a, int part, F run) {
+  auto with = [&](auto type, auto residual) __attribute__((always_inline)) {
+    if (WHOLE && part == LIN_WHOLE) run(type, lin_part<WHOLE ? LIN_WHOLE : LIN_ROWS>{}, residual);
+    else if (part >= LIN_ROWS) run(type, lin_part<LIN_ROWS>{}, residual);
+    else run(type, lin_part<LIN_EDGE>{}, residual);
+  };
+  auto typed = [&](auto type) __attribute__((always_inline)) {
+    if (a.residual) with(type, std::true_type{});
+    else with(type, std::false_type{});
+  };
+  if (a.dtype == BF16) typed(__bf16{});
+  else if (a.dtype == F32) typed(float{});
+  else typed(_Float16{});
 }
 
 // p[base + off], the base uniform and the lane's offset 32 bits of bytes: addressed without a 64-bit sum per lane
@@ -82,33 +99,41 @@ __device__ __forceinline__ void lin_channels(const LinearArgs& a, int nu, int nl
 #pragma unroll
   for (int e = 0; e < C; ++e) bias[e] = lin_f32(t[e]);
 }
-// The outputs of those channels of row m = mu + ml (mu uniform, ml < 32) from their sums.
+// The residual of channels n .. n+C-1 of row m = mu + ml.
 template <typename T, bool WHOLE, int C>
-__device__ __forceinline__ void lin_out(const LinearArgs& a, int mu, int ml, int nu, int nl, const float (&ws)[C],
-                                        const float (&bias)[C], const int (&sums)[C]) {
-  const int n = nu + nl;
-  const float xs = a.xs[mu + ml];
-  T* o = lin_at(static_cast<T*>(a.out), mu * a.ldo + nu, ml * (uint32_t)a.ldo + nl);
-  float v[C];
-#pragma unroll
-  for (int e = 0; e < C; ++e) v[e] = (float)sums[e] * (xs * ws[e]) + bias[e];
-  T t[C];
-  if (a.residual) {
-    const T* r = static_cast<const T*>(a.residual) + (mu + ml) * a.ldr + n;
-    if constexpr (WHOLE) __builtin_memcpy(t, r, sizeof(t));
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      if constexpr (!WHOLE) t[e] = n + e < a.n ? r[e] : T{};
-      v[e] += lin_f32(t[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < C; ++e) t[e] = (T)v[e];
-  if constexpr (WHOLE) __builtin_memcpy(o, t, sizeof(t));
+__device__ __forceinline__ void lin_residual(const LinearArgs& a, int mu, int ml, int n, T (&t)[C]) {
+  const T* r = static_cast<const T*>(a.residual) + (mu + ml) * a.ldr + n;
+  if constexpr (WHOLE) __builtin_memcpy(t, r, sizeof(t));
   else
 #pragma unroll
+    for (int e = 0; e < C; ++e) t[e] = n + e < a.n ? r[e] : T{};
+}
+// The outputs of channels nu + nl .. of row m = mu + ml (mu, nu uniform, ml < 32) from their sums; RESIDUAL: with `res`.
+template <typename T, bool WHOLE, bool RESIDUAL, int C>
+__device__ __forceinline__ void lin_out(const LinearArgs& a, int mu, int ml, int nu, int nl, float xs,
+                                        const float (&ws)[C], const float (&bias)[C], const T (&res)[C],
+                                        const int (&sums)[C]) {
+  T* o = lin_at(static_cast<T*>(a.out), mu * a.ldo + nu, ml * (uint32_t)a.ldo + nl);
+  T t[C];
+#pragma unroll
+  for (int e = 0; e < C; ++e) {
+    float v = __builtin_fmaf((float)sums[e] * xs, ws[e], bias[e]);
+    if constexpr (RESIDUAL) v += lin_f32(res[e]);
+    t[e] = (T)v;
+  }
+  if constexpr (WHOLE && sizeof(t) % 16 == 0) {
+    v4i q[sizeof(t) / 16];
+    __builtin_memcpy(q, t, sizeof(t));
+#pragma unroll
+    for (int e = 0; e < (int)sizeof(t) / 16; ++e)
+      __builtin_nontemporal_store(q[e], reinterpret_cast<v4i_any*>(o) + e);
+  } else if constexpr (WHOLE) {
+    __builtin_memcpy(o, t, sizeof(t));
+  } else {
+#pragma unroll
     for (int e = 0; e < C; ++e)
-      if (n + e < a.n) o[e] = t[e];
+      if (nu + nl + e < a.n) o[e] = t[e];
+  }
 }
 
 // the first `valid` of a chunk's 16 bytes (none for valid <= 0, all for valid >= 16)
@@ -201,12 +226,14 @@ __global__ __launch_bounds__(WAVES * 64) void dot_kernel(LinearArgs a) {
     int sum = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += red[w][m][r];
-    lin_typed(a.dtype, [&](auto type) {
+    const int one[1] = {sum};
+    lin_typed<false>(a, LIN_EDGE, [&](auto type, auto, auto res) {
       using T = decltype(type);
-      float v = (float)sum * (a.xs[m] * a.ws[n]);
-      if (a.bias) v += lin_f32(static_cast<const T*>(a.bias)[n]);
-      if (a.residual) v += lin_f32(static_cast<const T*>(a.residual)[m * a.ldr + n]);
-      static_cast<T*>(a.out)[m * a.ldo + n] = (T)v;
+      float ws[1], bias[1];
+      T r[1];
+      lin_channels<T, false>(a, 0, n, ws, bias);
+      if constexpr (decltype(res)::value) lin_residual<T, false>(a, m, 0, n, r);
+      lin_out<T, false, decltype(res)::value>(a, m, 0, 0, n, a.xs[m], ws, bias, r, one);
     });
   }
 }
@@ -239,17 +266,21 @@ __device__ __forceinline__ v4i lin_rsrc(const void* p) {
   return v4i{__builtin_amdgcn_readfirstlane((int)u), __builtin_amdgcn_readfirstlane((int)(u >> 32) & 0xffff),
              0x7fffffff, 0x00020000};
 }
-// 16 bytes a lane from byte `off` + `soff` of the rows to LDS byte `dst` + 16 * lane, awaited by lin_wait alone.  (The
-// builtin would make the compiler wait for every load in flight before it reads LDS again.)  The five wait states cover
-// a scalar operand that a vector instruction (readfirstlane) has just written: the compiler does not look into the asm
-// for that hazard.  Nothing else in these kernels uses m0.
+// 16 bytes a lane from byte `off` + `soff` of the rows to LDS byte `dst` + 16 * lane, if `mask` is
+// -1 and for no lane if it is 0 ( a load of no lanes is counted and done at once), awaited by lin_wait alone.  (The builtin would make the
+// compiler wait for every load in flight before it reads LDS again, and a branch around it would part the accumulators'
+// registers.)  Called with every lane active.  The wait states cover a scalar operand that a vector instruction
+// (readfirstlane) has just written: the compiler does not look into the asm for that hazard.  Nothing else in these
+// kernels uses m0.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void lin_lds_load(v4i rsrc, int off, int soff, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
-                   __builtin_amdgcn_readfirstlane(dst)),
-               "v"(off), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soff))
-               : "memory", "m0");
+__device__ __forceinline__ void lin_lds_load(v4i rsrc, int off, int soff, uint32_t dst, int mask) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\ts_nop 2\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
+      "s_mov_b64 exec, -1" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
+      "v"(off), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soff)),
+      "s"(__builtin_amdgcn_readfirstlane(mask))
+      : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t lin_lds_addr(const void* p) {
@@ -262,24 +293,25 @@ template <int BM, int BN, int WM, int WN, int S, int ST, bool SPLIT>
 __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, IM = TM / S, IN = TN / S;
   constexpr int CH = 64 / S;               // chunks of one MFMA (a lane's is L / S)
-  constexpr int KK = 8 / CH;               // MFMAs of a step
+  constexpr int KK = 8 / CH;               // operand sets of a step
   constexpr int PA = BM / 8, PB = BN / 8;  // loads (8 rows each) of a step
   constexpr int LA = (PA + WAVES - 1) / WAVES, LB = (PB + WAVES - 1) / WAVES, LPS = LA + LB;
   constexpr int RUN = 64 / S * 4;          // a lane's rows of a block come in runs of four, RUN apart
   constexpr bool ROWS = !SPLIT && S == 32;  // outputs pass through LDS
+  constexpr int AREAS = IN * IM >= 16 ? 2 : 1;  // 4 KiB each a wave (two would cost the small forms a workgroup a CU)
   static_assert(TM % S == 0 && TN % S == 0 && BM % 8 == 0 && BN % 8 == 0, "whole MFMA blocks");
   static_assert(ST >= 2 && ST <= 4 && KK % 2 == 0, "buffers");
   using M = MfmaI8<S>;
   constexpr int BUF = (BM + BN) * LIN_KS;
   __shared__ __align__(16) int8_t bufs[ST][BUF];
-  __shared__ __align__(16) int8_t rows[ROWS ? WAVES : 1][ROWS ? 4096 : 16];
+  __shared__ __align__(16) int8_t rows[ROWS ? WAVES : 1][ROWS ? AREAS * 4096 : 16];
 
   const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM, lr = L % S, lc = L / S;
   const int total = a.tiles_m * a.tiles_n * a.splits, steps = (a.k + LIN_KS - 1) / LIN_KS;
   const int last_chunk = (a.k - 1) & ~15;
   const int full = a.k / LIN_KS;         // steps whose 8 chunks all lie in the row
-  const int chunk = (L & 7) ^ (L >> 3);  // (the row's low bits are L >> 3)
+  const int chunk = (L & 7) ^ (L >> 3);  // this lane's of a load (the row's low bits are L >> 3)
 
   // The tile: its place, its steps, and this wave's loads: the 8-row pieces and this lane's byte offsets at K = 0 (a wave
   // without a piece of its own repeats the last one, so that every wave counts the same loads).
@@ -312,39 +344,55 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
     for (int i = 0; i < LB; ++i)
       vw[i] = min(min(wave + i * WAVES, PB - 1) * 8 + (L >> 3), a.n - 1 - n0) * (int)a.ldw;
   };
-  auto issue = [&](int8_t* buf, int s) __attribute__((always_inline)) {
-    const int koff = s < full ? chunk * 16 : min(s * LIN_KS + chunk * 16, last_chunk) - s * LIN_KS;
+  auto issue_piece = [&](int8_t* buf, int s, int koff, int i, int mask) __attribute__((always_inline)) {
     const uint32_t dst = lin_lds_addr(buf);
+    if (i < LA)
+      lin_lds_load(rx, vx[i] + koff, s * LIN_KS, dst + min(wave + i * WAVES, PA - 1) * 1024, mask);
+    else
+      lin_lds_load(rw, vw[i - LA] + koff, s * LIN_KS, dst + BM * LIN_KS + min(wave + (i - LA) * WAVES, PB - 1) * 1024,
+                   mask);
+  };
+  auto issue = [&](int8_t* buf, int s, bool some) __attribute__((always_inline)) {
+    const int koff = s < full ? chunk * 16 : min(s * LIN_KS + chunk * 16, last_chunk) - s * LIN_KS;
 #pragma unroll
-    for (int i = 0; i < LA; ++i)
-      lin_lds_load(rx, vx[i] + koff, s * LIN_KS, dst + min(wave + i * WAVES, PA - 1) * 1024);
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-      lin_lds_load(rw, vw[i] + koff, s * LIN_KS, dst + BM * LIN_KS + min(wave + i * WAVES, PB - 1) * 1024);
+    for (int i = 0; i < LPS; ++i) issue_piece(buf, s, koff, i, some ? -1 : 0);
   };
   auto start = [&]() __attribute__((always_inline)) {  // the first ST steps' loads; the step that ends inside its 128 bytes first
 #pragma unroll
-    for (int u = 0; u < ST - 1; ++u)
-      if (s0 + u < whole) issue(bufs[u], s0 + u);
-    if (tail) issue(bufs[ST - 1], full);
-    else if (s0 + ST - 1 < whole) issue(bufs[ST - 1], s0 + ST - 1);
+    for (int u = 0; u < ST - 1; ++u) issue(bufs[u], s0 + u, s0 + u < whole);
+    if (tail) issue(bufs[ST - 1], full, true);
+    else issue(bufs[ST - 1], s0 + ST - 1, s0 + ST - 1 < whole);
   };
 
   typename M::acc_t acc[IN][IM];
   const int xa = (wm * TM + lr) * LIN_KS, wa = BM * LIN_KS + (wn * TN + lr) * LIN_KS, sw = lr & 7;
   v4i fx[2][IM], fw[2][IN];
-  auto read = [&](const int8_t* buf, int kk) __attribute__((always_inline)) {
+  auto read_one = [&](const int8_t* buf, int kk, int r) __attribute__((always_inline)) {
     const int slot = ((kk * CH + lc) ^ sw) * 16;
-#pragma unroll
-    for (int i = 0; i < IM; ++i) fx[kk & 1][i] = *reinterpret_cast<const v4i*>(buf + xa + i * S * LIN_KS + slot);
-#pragma unroll
-    for (int i = 0; i < IN; ++i) fw[kk & 1][i] = *reinterpret_cast<const v4i*>(buf + wa + i * S * LIN_KS + slot);
+    if (r < IM) fx[kk & 1][r] = *reinterpret_cast<const v4i*>(buf + xa + r * S * LIN_KS + slot);
+    else fw[kk & 1][r - IM] = *reinterpret_cast<const v4i*>(buf + wa + (r - IM) * S * LIN_KS + slot);
   };
-  auto multiply = [&](int kk) __attribute__((always_inline)) {
+  auto read = [&](const int8_t* buf, int kk) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < IN; ++i)
+    for (int r = 0; r < IM + IN; ++r) read_one(buf, kk, r);
+  };
+  // The MFMAs of one operand set; between them, one or two at a time, the reads of the next set (rkk of rbuf) and loads
+  // i0 .. i1-1 of step istep into ibuf.  In bursts those would hold the wave, whose instructions issue in order, and the
+  // matrix cores with it: every wave of the workgroup is at the same place.
+  auto phase = [&](int kk, const int8_t* rbuf, int rkk, int8_t* ibuf, int istep, int mask, int i0, int i1)
+      __attribute__((always_inline)) {
+    constexpr int NM = IN * IM, NR = IM + IN;
 #pragma unroll
-      for (int j = 0; j < IM; ++j) acc[i][j] = M::run(fw[kk & 1][i], fx[kk & 1][j], acc[i][j]);
+    for (int q = 0; q < NM; ++q) {
+      const int i = q / IM, j = q % IM;
+      acc[i][j] = M::run(fw[kk & 1][i], fx[kk & 1][j], acc[i][j]);
+#pragma unroll
+      for (int r = q * NR / NM; r < (q + 1) * NR / NM; ++r) read_one(rbuf, rkk, r);
+#pragma unroll
+      for (int p = i0 + q * (i1 - i0) / NM; p < i0 + (q + 1) * (i1 - i0) / NM; ++p)
+        issue_piece(ibuf, istep, chunk * 16, p, mask);
+      __builtin_amdgcn_sched_barrier(0);  // (the compiler would gather them again)
+    }
   };
 
   int t = blockIdx.x;
@@ -363,43 +411,41 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
 #pragma unroll
         for (int i = 0; i < IM; ++i)
           fx[kk & 1][i] = lin_mask(fx[kk & 1][i], a.k - full * LIN_KS - (kk * CH + lc) * 16);
-        multiply(kk);
+#pragma unroll
+        for (int i = 0; i < IN; ++i)
+#pragma unroll
+          for (int j = 0; j < IM; ++j) acc[i][j] = M::run(fw[kk & 1][i], fx[kk & 1][j], acc[i][j]);
       }
       lin_wait<0>();
-      if (s0 + ST - 1 < whole) issue(bufs[ST - 1], s0 + ST - 1);
-    } else if (first && s0 + ST - 1 < whole) {
+      issue(bufs[ST - 1], s0 + ST - 1, s0 + ST - 1 < whole);
+    } else if (first) {
       lin_wait<(ST - 1) * LPS>();
     } else {
       lin_wait<0>();  // (after a first tile the counter holds its stores too)
     }
-    // Step s: the operands of one MFMA are read while the one before runs.  Before the last, every operand of the step
-    // is in registers: the workgroup meets, its buffer takes step s + ST, and the next step's first operands are read.
-    if (s0 < whole) read(bufs[0], 0);
+    // Step s: an operand set is read while the one before is multiplied.  Before the last set's MFMAs every operand of
+    // the step is in registers: the workgroup meets, and the step's buffer takes step s + ST, half of its loads among
+    // those MFMAs and half among the next step's first.  (Past the last step the reads find what the buffer holds, and
+    // nothing is loaded.)
+    read(bufs[0], 0);
     for (int s = s0; s < whole; s += ST) {
 #pragma unroll
       for (int u = 0; u < ST; ++u) {
         if (s + u < whole) {
+          const int now = s + u;
+          phase(0, bufs[u], 1, bufs[(u + ST - 1) % ST], now - 1 + ST, now > s0 && now - 1 + ST < whole ? -1 : 0,
+                LPS / 2, LPS);
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            if (kk + 1 < KK) {
-              read(bufs[u], kk + 1);
-            } else if (s + u + 1 < whole) {
-              if (s + u + ST - 1 < whole) lin_wait<(ST - 2) * LPS>();
-              else lin_wait<0>();
-              if (s + u + ST < whole) issue(bufs[u], s + u + ST);
-              read(bufs[(u + 1) % ST], 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);  // (the compiler would read each operand right before its use)
-            multiply(kk);
-            __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int kk = 1; kk + 1 < KK; ++kk) phase(kk, bufs[u], kk + 1, nullptr, 0, 0, 0, 0);
+          lin_wait<(ST - 2) * LPS>();
+          phase(KK - 1, bufs[(u + 1) % ST], 0, bufs[u], now + ST, now + ST < whole ? -1 : 0, 0, LPS / 2);
         }
       }
     }
 
     // a lane's column of block (i, j) is m; its rows are n
     const int tm0 = m0 + wm * TM, tn0 = n0 + wn * TN, tsplit = split;
-    const bool whole_n = n0 + BN <= a.n;
+    const int exists = n0 + BN > a.n ? LIN_EDGE : m0 + BM > a.m ? LIN_ROWS : LIN_WHOLE;
     t += gridDim.x;
     if (t < total) {
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave has read its last operands
@@ -427,40 +473,63 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
         }
       }
     } else {
-      auto write = [&](auto type, auto whole_tile) __attribute__((always_inline)) {
+      auto write = [&](auto type, auto part, auto with_residual) __attribute__((always_inline)) {
         using T = decltype(type);
-        constexpr bool WHOLE = decltype(whole_tile)::value;
+        constexpr bool WHOLE = decltype(part)::value >= LIN_ROWS, ALL = decltype(part)::value == LIN_WHOLE;
+        constexpr bool RESIDUAL = decltype(with_residual)::value;
         if constexpr (ROWS) {
-          // A block's sums pass through the wave's own 4 KiB of LDS, row m at 128 bytes, 16-byte piece p at slot
-          // p ^ (m & 7): four lanes then hold a row's 32 channels, eight each, with one set of scales for all rows.
-          int8_t* own = rows[wave];
+          // A block's sums pass through 4 KiB of the wave's own LDS, row m at 128 bytes, 16-byte piece p at slot
+          // p ^ (m & 7): four lanes then hold a row's 32 channels, eight each, with one set of scales for all rows.  With
+          // two such areas a block is put while the one before is read, its residual's loads ahead of that one's stores.
+          constexpr int NB = IN * IM;
           const int row = L >> 2, c8 = (L & 3) * 8;
+          float xs[IM][2], ws[IN][8], bias[IN][8];
 #pragma unroll
-          for (int i = 0; i < IN; ++i) {
-            float ws[8], bias[8];
-            lin_channels<T, WHOLE>(a, tn0 + i * S, c8, ws, bias);
+          for (int j = 0; j < IM; ++j)
 #pragma unroll
-            for (int j = 0; j < IM; ++j) {
+            for (int h = 0; h < 2; ++h) xs[j][h] = a.xs[min(tm0 + j * S + h * 16 + row, a.m - 1)];
 #pragma unroll
-              for (int g = 0; g < S / RUN; ++g)
-                *reinterpret_cast<v4i*>(own + lr * 128 + ((2 * g + lc) ^ (lr & 7)) * 16) =
-                    v4i{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+          for (int i = 0; i < IN; ++i) lin_channels<T, WHOLE>(a, tn0 + i * S, c8, ws[i], bias[i]);
+          T res[2][2][8];
+          auto put = [&](int b) __attribute__((always_inline)) {
+            const int i = b / IM, j = b % IM;
+            int8_t* own = rows[wave] + b % AREAS * 4096;
+#pragma unroll
+            for (int g = 0; g < S / RUN; ++g)
+              *reinterpret_cast<v4i*>(own + lr * 128 + ((2 * g + lc) ^ (lr & 7)) * 16) =
+                  v4i{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            if constexpr (RESIDUAL) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const int mu = tm0 + j * S + h * 16, nu = tn0 + i * S;
-                const int8_t* src = own + (h * 16 + row) * 128;
-                v4i v[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  v[e] = *reinterpret_cast<const v4i*>(src + ((2 * (L & 3) + e) ^ (row & 7)) * 16);
-                if (mu + row < a.m) {
-                  const int sums[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
-                  lin_out<T, WHOLE>(a, mu, row, nu, c8, ws, bias, sums);
-                }
+                const int mu = tm0 + j * S + h * 16;
+                if (ALL || mu + row < a.m) lin_residual<T, WHOLE>(a, mu, row, tn0 + i * S + c8, res[b & 1][h]);
               }
+            }
+          };
+          if (AREAS == 2) put(0);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            if (AREAS == 1) put(b);
+            else if (b + 1 < NB) put(b + 1);
+            const int i = b / IM, j = b % IM;
+            const int8_t* own = rows[wave] + b % AREAS * 4096;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int mu = tm0 + j * S + h * 16;
+              const int8_t* src = own + (h * 16 + row) * 128;
+              v4i v[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                v[e] = *reinterpret_cast<const v4i*>(src + ((2 * (L & 3) + e) ^ (row & 7)) * 16);
+              const int sums[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+              if (ALL || mu + row < a.m)
+                lin_out<T, WHOLE, RESIDUAL>(a, mu, row, tn0 + i * S, c8, xs[j][h], ws[i], bias[i], res[b & 1][h], sums);
             }
           }
         } else {
+          float xs[IM];
+#pragma unroll
+          for (int j = 0; j < IM; ++j) xs[j] = a.xs[min(tm0 + j * S + lr, a.m - 1)];
 #pragma unroll
           for (int i = 0; i < IN; ++i)
 #pragma unroll
@@ -471,15 +540,16 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
 #pragma unroll
               for (int j = 0; j < IM; ++j) {
                 const int sums[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                if (tm0 + j * S + lr < a.m) lin_out<T, WHOLE>(a, tm0 + j * S, lr, nu, 4 * lc, ws, bias, sums);
+                if (ALL || tm0 + j * S + lr < a.m) {
+                  T res[4];
+                  if constexpr (RESIDUAL) lin_residual<T, WHOLE>(a, tm0 + j * S, lr, nu + 4 * lc, res);
+                  lin_out<T, WHOLE, RESIDUAL>(a, tm0 + j * S, lr, nu, 4 * lc, xs[j], ws, bias, res, sums);
+                }
               }
             }
         }
       };
-      lin_typed(a.dtype, [&](auto type) __attribute__((always_inline)) {
-        if (whole_n) write(type, std::true_type{});
-        else write(type, std::false_type{});
-      });
+      lin_typed(a, exists, write);
     }
     if (t >= total) return;
   }
@@ -507,16 +577,14 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += t[e];
   }
-  lin_typed(a.dtype, [&](auto type) {
+  lin_typed<false>(a, n + 4 <= a.n ? LIN_ROWS : LIN_EDGE, [&](auto type, auto part, auto res) {
     using T = decltype(type);
+    constexpr bool WHOLE = decltype(part)::value >= LIN_ROWS;
     float ws[4], bias[4];
-    if (n + 4 <= a.n) {
-      lin_channels<T, true>(a, 0, n, ws, bias);
-      lin_out<T, true>(a, m, 0, 0, n, ws, bias, v);
-    } else {
-      lin_channels<T, false>(a, 0, n, ws, bias);
-      lin_out<T, false>(a, m, 0, 0, n, ws, bias, v);
-    }
+    T r[4];
+    lin_channels<T, WHOLE>(a, 0, n, ws, bias);
+    if constexpr (decltype(res)::value) lin_residual<T, WHOLE>(a, m, 0, n, r);
+    lin_out<T, WHOLE, decltype(res)::value>(a, m, 0, 0, n, a.xs[m], ws, bias, r, v);
   });
 }
 
@@ -534,17 +602,17 @@ struct LinearForm {
   double step, fixed;
 };
 constexpr LinearForm LIN_FORMS[] = {
-    {16, 64, 3, 0.13, 0.7},   {32, 64, 3, 0.20, 1.3},   {64, 64, 2, 0.32, 1.4},
-    {128, 128, 2, 0.70, 3.4},  // two buffers, two workgroups a CU
-    {128, 128, 1, 0.70, 3.0},  // four buffers: for fewer tiles than CUs
-    {256, 256, 1, 0.90, 7.4},
+    {16, 64, 3, 0.171, 0.8},  {32, 64, 3, 0.15, 1.4},   {64, 64, 2, 0.29, 0.7},
+    {128, 128, 2, 0.73, 3.9},  // two buffers, two workgroups a CU
+    {128, 128, 1, 0.55, 5.5},  // four buffers: for fewer tiles than CUs
+    {256, 256, 1, 1.0, 5.5},
 };
 
 // The form and the split that this model of their time holds fastest: rounds of resident workgroups, each step bound by
-// its own latency, by the bytes that a CU takes from its L2 (63 GB/s) or by the matrix cores (12.7 Top/s a CU); never
-// below the stream of both operands (5.75 TB/s); a split adds its launch and its partials' way through memory.  Fitted
-// to 2,500 timings of 121 shapes (5 to 4,096 rows, 640 to 37,888 channels, K 1,000 to 18,944): its choice takes 0.5% more
-// than the fastest of all forms and splits on the mean, 11% at most.
+// its own latency, by the bytes that a CU takes from its L2 (64.7 GB/s) or by the matrix cores (9.8 Top/s a CU); never
+// below the stream of both operands (6 TB/s); a split adds its launch and its partials' way through memory.  Fitted to
+// 2,700 timings of 149 shapes (5 to 8,192 rows, 640 to 37,888 channels, K 1,000 to 18,944): its choice takes 0.2% more
+// than the fastest of all forms and splits on the mean, 5% at most.
 inline LinearPlan linear_plan(int m, int n, int k, int cus) {
   const int steps = (k + LIN_KS - 1) / LIN_KS;
   LinearPlan best{};
@@ -554,12 +622,12 @@ inline LinearPlan linear_plan(int m, int n, int k, int cus) {
   // for 8; the 16-row tile 15-16 us at any count).
   if (m <= 4) return best;
   double least = 1e300;
-  const double stream = ((double)n * k + (double)m * k) / 5.75e6;
+  const double stream = ((double)n * k + (double)m * k) / 6.0e6;
   for (int f = 0; f < 6; ++f) {
     const LinearForm& form = LIN_FORMS[f];
     const int64_t tiles = (int64_t)((m + form.bm - 1) / form.bm) * ((n + form.bn - 1) / form.bn);
     const int64_t slots = (int64_t)cus * form.resident;
-    const double bytes = (form.bm + form.bn) * LIN_KS / 63e3, ops = 2.0 * form.bm * form.bn * LIN_KS / 12.7e6;
+    const double bytes = (form.bm + form.bn) * LIN_KS / 64.7e3, ops = 2.0 * form.bm * form.bn * LIN_KS / 9.8e6;
     for (int want = 1; want <= 16 && (want == 1 || (steps >= 4 * want && tiles * want <= 5 * (int64_t)cus)); ++want) {
       const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
       const int64_t work = tiles * splits, rounds = work / slots;
@@ -567,7 +635,7 @@ inline LinearPlan linear_plan(int m, int n, int k, int cus) {
       double t = rounds * (per * std::max(form.step, form.resident * std::max(bytes, ops)) + form.fixed);
       if (left) t += per * std::max(form.step, left * std::max(bytes, ops)) + form.fixed;
       t = std::max(t, stream);
-      if (splits > 1) t += 2.2 + 0.17 * splits + 8.0 * splits * m * n / 3.4e6;
+      if (splits > 1) t += 2.6 + 0.44 * splits + 8.0 * splits * m * n / 3.77e6;
       if (t < least) {
         least = t;
         best = {f + 1, form.bm, form.bn, splits, per, INT32_MAX};
@@ -606,10 +674,10 @@ inline void launch_linear(LinearArgs a, const LinearPlan& p, hipStream_t s) {
   switch (p.kind) {
     case 1: launch_tile<16, 64, 1, 4, 16, 4>(a, p.groups, s); break;
     case 2: launch_tile<32, 64, 1, 4, 16, 4>(a, p.groups, s); break;
-    case 3: launch_tile<64, 64, 2, 2, 32, 3>(a, p.groups, s); break;
+    case 3: launch_tile<64, 64, 2, 2, 16, 4>(a, p.groups, s); break;
     case 4: launch_tile<128, 128, 2, 2, 32, 2>(a, p.groups, s); break;
     case 5: launch_tile<128, 128, 2, 2, 32, 4>(a, p.groups, s); break;
-    default: launch_tile<256, 256, 2, 4, 32, 2>(a, p.groups, s); break;
+    default: launch_tile<256, 256, 2, 2, 32, 2>(a, p.groups, s); break;
   }
   if (p.splits > 1) {
     const int64_t quads = (int64_t)a.m * ((a.n + 3) / 4);
