@@ -150,6 +150,20 @@ class Module:
             with torch.cuda.device(index):
                 self._call(fn, *args, stream)
 
+    def _launch_for(self, x, fn, *args):
+        """``fn(*args, stream)`` on the current stream of ``x``'s device, with that device current: ``_launch`` for ops
+        whose host time is most of a small call (the stream's handle without a Stream object around it: 1 us less)."""
+        index = x.get_device()
+        if index < 0:
+            raise ValueError(f"Expected a cuda device, but got: {x.device}")
+        if index == torch._C._cuda_getDevice():
+            failed = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                failed = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if failed:
+            raise RuntimeError(self.lib.tri_last_error().decode())
+
     # -------------------------------------------------------------- prepare_qk
     @staticmethod
     def _check_rows(q, k):
@@ -549,7 +563,7 @@ class Module:
     def _check_float_rows(x, what, like=None):
         if x.dim() != 2 or x.dtype not in _DTYPES or (x.stride(1) != 1 and x.size(1) != 1):
             raise RuntimeError(f"{what}: fp32, bf16 or fp16 rows [M,K] with contiguous features")
-        if like is not None and (x.shape != like.shape or x.dtype != like.dtype or x.device != like.device):
+        if like is not None and (x.shape != like.shape or x.dtype != like.dtype or x.get_device() != like.get_device()):
             raise RuntimeError(f"{what}: not of the other rows' shape, type and device")
 
     @staticmethod
@@ -566,13 +580,13 @@ class Module:
         self._quantize_rows(x, codes, codes.stride(0), scales)
 
     def _quantize_rows(self, x, codes, ldc, scales):
-        self._launch(x.device, self.lib.tri_quantize_rows, x.data_ptr(), x.stride(0), _DTYPES[x.dtype], x.size(0),
+        self._launch_for(x, self.lib.tri_quantize_rows, x.data_ptr(), x.stride(0), _DTYPES[x.dtype], x.size(0),
                      x.size(1), codes.data_ptr(), ldc, scales.data_ptr())
 
     def _check_norm(self, x, residual, weight):
         self._check_float_rows(x, "rms_norm_quant")
         _check(weight.dtype == x.dtype and weight.dim() == 1 and weight.numel() == x.size(1) and
-               weight.is_contiguous() and weight.device == x.device, "rms_norm_quant: weight [K] of x's type, on its device")
+               weight.is_contiguous() and weight.get_device() == x.get_device(), "rms_norm_quant: weight [K] of x's type, on its device")
         if residual is not None:
             self._check_float_rows(residual, "rms_norm_quant: residual", x)
 
@@ -588,7 +602,7 @@ class Module:
                              0 if hidden is None else hidden.stride(0))
 
     def _rms_norm_quant(self, x, residual, weight, eps, codes, ldc, scales, hidden, ldh):
-        self._launch(x.device, self.lib.tri_rms_norm_quant, x.data_ptr(), x.stride(0), _ptr(residual),
+        self._launch_for(x, self.lib.tri_rms_norm_quant, x.data_ptr(), x.stride(0), _ptr(residual),
                      0 if residual is None else residual.stride(0), weight.data_ptr(), _DTYPES[x.dtype], x.size(0),
                      x.size(1), eps, codes.data_ptr(), ldc, scales.data_ptr(), _ptr(hidden), ldh)
 
@@ -603,41 +617,39 @@ class Module:
         self._silu_mul_quant(gate, up, codes, codes.stride(0), scales)
 
     def _silu_mul_quant(self, gate, up, codes, ldc, scales):
-        self._launch(gate.device, self.lib.tri_silu_mul_quant, gate.data_ptr(), gate.stride(0), up.data_ptr(),
+        self._launch_for(gate, self.lib.tri_silu_mul_quant, gate.data_ptr(), gate.stride(0), up.data_ptr(),
                      up.stride(0), _DTYPES[gate.dtype], gate.size(0), gate.size(1), codes.data_ptr(), ldc,
                      scales.data_ptr())
 
     def int8_linear_workspace(self, m, n, k, device) -> int:
         """Bytes of workspace ``int8_linear`` needs for a product of [m,k] and [n,k] codes on ``device``."""
-        index = device.index if device.index is not None else torch.cuda.current_device()
-        found = self._workspaces.get((m, n, k, index))
+        found = self._workspaces.get((m, n, k, device))
         if found is None:
             size = ctypes.c_int64(0)
-            with torch.cuda.device(index):
+            with torch.cuda.device(device):
                 self._call(self.lib.tri_int8_linear_workspace, m, n, k, ctypes.byref(size))
             if len(self._workspaces) >= 4096:
                 self._workspaces.clear()
-            found = self._workspaces[(m, n, k, index)] = int(size.value)
+            found = self._workspaces[(m, n, k, device)] = int(size.value)
         return found
 
     @staticmethod
     def _check_linear(x, xs, w, ws, bias, residual, dtype):
-        k, device = x.size(1), x.device
-        _check(x.dtype == w.dtype == torch.int8 and w.dim() == 2 and w.size(1) == k and w.device == device and
+        (m, k), n, device = x.shape, w.size(0), x.get_device()
+        _check(x.dtype == w.dtype == torch.int8 and w.dim() == 2 and w.size(1) == k and w.get_device() == device and
                (k == 1 or (x.stride(1) == 1 and w.stride(1) == 1)),
                "int8_linear: int8 codes [M,K] and [N,K] with contiguous features, on one device")
-        n = w.size(0)
-        _check(xs.dtype == ws.dtype == torch.float32 and xs.numel() == x.size(0) and ws.numel() == n and
-               xs.is_contiguous() and ws.is_contiguous() and xs.device == device and ws.device == device,
+        _check(xs.dtype == ws.dtype == torch.float32 and xs.numel() == m and ws.numel() == n and
+               xs.is_contiguous() and ws.is_contiguous() and xs.get_device() == device and ws.get_device() == device,
                "int8_linear: scales fp32 [M] and [N], contiguous, on the codes' device")
         _check(dtype in _DTYPES, "int8_linear: out fp32, bf16 or fp16")
-        _check(bias is None or (bias.dtype == dtype and bias.dim() == 1 and bias.numel() == n and
-                                bias.is_contiguous() and bias.device == device),
-               "int8_linear: bias [N] of out's type, on the codes' device")
-        _check(residual is None or (residual.dtype == dtype and residual.dim() == 2 and
-                                    residual.size(0) == x.size(0) and residual.size(1) == n and
-                                    (residual.stride(1) == 1 or n == 1) and residual.device == device),
-               "int8_linear: residual [M,N] of out's type, with contiguous features, on the codes' device")
+        if bias is not None:
+            _check(bias.dtype == dtype and bias.dim() == 1 and bias.numel() == n and bias.is_contiguous() and
+                   bias.get_device() == device, "int8_linear: bias [N] of out's type, on the codes' device")
+        if residual is not None:
+            _check(residual.dtype == dtype and residual.dim() == 2 and residual.size(0) == m and
+                   residual.size(1) == n and (residual.stride(1) == 1 or n == 1) and residual.get_device() == device,
+                   "int8_linear: residual [M,N] of out's type, with contiguous features, on the codes' device")
 
     def int8_linear(self, x, xs, w, ws, bias, residual, out, workspace):
         """``out = xs[:, None] * ws * (x @ w.T) + bias + residual`` of int8 codes ``x`` [M,K] and ``w`` [N,K]
@@ -654,7 +666,7 @@ class Module:
     def _int8_linear(self, x, xs, w, ws, bias, residual, out, ldo, workspace):
         m, n = x.size(0), w.size(0)
         # (a single row's stride is never applied)
-        self._launch(x.device, self.lib.tri_int8_linear, x.data_ptr(), x.stride(0) if m > 1 else 0, xs.data_ptr(),
+        self._launch_for(x, self.lib.tri_int8_linear, x.data_ptr(), x.stride(0) if m > 1 else 0, xs.data_ptr(),
                      w.data_ptr(), w.stride(0) if n > 1 else 0, ws.data_ptr(), _ptr(bias), _ptr(residual),
                      0 if residual is None else residual.stride(0), out.data_ptr(), ldo, _DTYPES[out.dtype], m, n,
                      x.size(1), _ptr(workspace), 0 if workspace is None else workspace.nbytes)

@@ -45,10 +45,10 @@ def _serving(what, *tensors):
 
 def _outputs(x):
     """Codes like ``x`` [..., K] at a row stride of a multiple of 16 bytes, the stride, and the rows' scales."""
-    k = x.size(-1)
+    *lead, k = x.shape
     ld = k + -k % 16
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    codes = torch.empty((*x.shape[:-1], ld), dtype=torch.int8, device=x.device)
+    scales = x.new_empty(lead, dtype=torch.float32)
+    codes = x.new_empty((*lead, ld), dtype=torch.int8)
     return codes if ld == k else codes[..., :k], ld, scales
 
 
@@ -82,7 +82,7 @@ def rms_norm_quant(x, weight, eps, residual=None):
     module._check_norm(rows, other, weight)
     codes, ld, scales = _outputs(x)
     if residual is not None:
-        hidden = sums = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        hidden = sums = x.new_empty(x.shape)
     module._rms_norm_quant(rows, other, weight, eps, codes, ld, scales, sums, x.size(-1))
     return codes, scales, hidden
 
@@ -111,22 +111,23 @@ def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, 
     if scales.requires_grad or (bias is not None and bias.requires_grad) or \
             (residual is not None and residual.requires_grad):
         _serving("int8_linear", scales, bias, residual)
-    x = _rows(codes, "int8_linear")
-    if scales.shape != codes.shape[:-1] or weight.dim() != 2 or weight.size(1) != x.size(1):
+    *lead, k = shape = list(codes.shape)
+    if list(scales.shape) != lead or weight.dim() != 2 or weight.size(1) != k:
         raise RuntimeError(f"int8_linear: codes {tuple(codes.shape)}, scales {tuple(scales.shape)} and weight "
                            f"{tuple(weight.shape)} do not go together ([..., K], [...], [N, K])")
-    m, n = x.size(0), weight.size(0)
-    shape = (*codes.shape[:-1], n)
+    x = _rows(codes, "int8_linear")
+    shape[-1] = n = weight.size(0)
     other = None
     if residual is not None:
-        if residual.shape != shape:
-            raise RuntimeError(f"int8_linear: residual {tuple(residual.shape)} unlike the output {shape}")
+        if list(residual.shape) != shape:
+            raise RuntimeError(f"int8_linear: residual {tuple(residual.shape)} unlike the output {tuple(shape)}")
         other = _rows(residual, "int8_linear: residual")
     module = load_extension()
     module._check_linear(x, scales, weight, weight_scales, bias, other, out_dtype)
-    out = torch.empty(shape, dtype=out_dtype, device=x.device)
-    size = module.int8_linear_workspace(m, n, x.size(1), x.device) if m else 0
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    out = codes.new_empty(shape, dtype=out_dtype)
+    m = x.size(0)
+    size = module.int8_linear_workspace(m, n, k, codes.device) if m > 4 else 0  # (fewer rows are never split over K)
+    workspace = codes.new_empty(size, dtype=torch.uint8) if size else None
     module._int8_linear(x, scales, weight, weight_scales, bias, other, out, n, workspace)
     return out
 
