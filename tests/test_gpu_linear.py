@@ -113,6 +113,19 @@ def test_many_rows(module, m, k):
     check_codes(*Q.quantize_rows(x), x.double(), 127 * 5 * U, 2 * U)
 
 
+@pytest.mark.parametrize("k", [100, 512, 900, 2048, 2049, 4096, 9000, 18944, 30000, 33001])
+@pytest.mark.parametrize("place", ["x", "residual"])
+def test_the_sum_may_take_its_operands_place(module, k, place):
+    g = gen(k)
+    for m in (1, 7):
+        x, r = hidden(g, m, k, torch.bfloat16), hidden(g, m, k, torch.bfloat16)
+        w = (1 + 0.3 * torch.randn(k, generator=g, device=DEV)).bfloat16()
+        codes, scales, h = Q.rms_norm_quant(x, w, 1e-6, residual=r)
+        c, s = torch.empty(m, k, dtype=torch.int8, device=DEV), torch.empty(m, device=DEV)
+        module.rms_norm_quant(x, r, w, 1e-6, c, s, x if place == "x" else r)
+        assert torch.equal(x if place == "x" else r, h) and torch.equal(c, codes) and torch.equal(s, scales)
+
+
 def test_silu_of_far_negative_gates(module):
     # rows of negative gates alone: their own scale, down to where exp overflows (values of 0)
     gate = torch.stack([torch.linspace(-b, -b / 2, 300, device=DEV) for b in (1.0, 20.0, 60.0, 87.0, 300.0, 3e38)])
@@ -220,6 +233,21 @@ def test_int8_linear(module, m, n, k):
 def test_int8_linear_many_tiles(module, m, n, k):
     x, xs, w, ws, b, r = operands(m, m, n, k, torch.bfloat16, True, True)
     check_linear(x, xs, w, ws, b, r, torch.bfloat16, Q.int8_linear(x, xs, w, ws, b, r))
+
+
+@pytest.mark.parametrize("k", [64, 128, 160, 256, 384, 512, 640, 700])
+@pytest.mark.parametrize("m,n", [(5, 300), (20, 2000), (40, 9000), (100, 4608), (300, 3000), (700, 5000), (1500, 6100),
+                                 (4097, 5889)])
+def test_few_steps(module, m, n, k):
+    """Every tile form with fewer steps than buffers, as many, and a few more (sums below 2^24: fp32 products are exact)."""
+    x, xs, w, ws, b, r = operands(m + k, m, n, k, torch.bfloat16, True, True)
+    y = (x.float() @ w.float().t()).double()
+    assert torch.equal(y, y.round())
+    y = y * xs.double()[:, None] * ws.double()
+    size = y.abs() + b.double().abs() + r.double().abs()
+    y = y + b.double() + r.double()
+    tol = 5 * U * size + torch.finfo(torch.bfloat16).eps / 2 * (y.abs() + 5 * U * size)
+    assert ((Q.int8_linear(x, xs, w, ws, b, r).double() - y).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("m", [1, 4, 16, 40, 200])

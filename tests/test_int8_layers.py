@@ -107,6 +107,11 @@ def test_refusals_leave_the_model_alone(plain):
         M.use_int8_layers(model)
     assert type(model.model.layers[0].self_attn.q_proj) is torch.nn.Linear
     model = tiny("llama")
+    model.model.layers[1].mlp.down_proj.bfloat16()
+    with pytest.raises(ValueError, match="one type"):
+        M.use_int8_layers(model)
+    assert type(model.model.layers[0].self_attn.q_proj) is torch.nn.Linear
+    model = tiny("llama")
     M.use_int8_layers(model)
     with pytest.raises(ValueError, match="already"):
         M.use_int8_layers(model)

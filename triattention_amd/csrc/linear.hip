@@ -267,9 +267,9 @@ __device__ __forceinline__ v4i lin_rsrc(const void* p) {
              0x7fffffff, 0x00020000};
 }
 // 16 bytes a lane from byte `off` + `soff` of the rows to LDS byte `dst` + 16 * lane, if `mask` is
-// -1 and for no lane if it is 0 ( a load of no lanes is counted and done at once), awaited by lin_wait alone.  (The builtin would make the
-// compiler wait for every load in flight before it reads LDS again, and a branch around it would part the accumulators'
-// registers.)  Called with every lane active.  The wait states cover a scalar operand that a vector instruction
+// -1 and for no lane if it is 0, awaited by lin_wait alone.  (The builtin would make the compiler wait for every load in
+// flight before it reads LDS again, and a branch around the load would part the accumulators' registers.)  Called with
+// every lane active.  The wait states cover a scalar operand that a vector instruction
 // (readfirstlane) has just written: the compiler does not look into the asm for that hazard.  Nothing else in these
 // kernels uses m0.
 #pragma clang diagnostic push
@@ -418,10 +418,10 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
       }
       lin_wait<0>();
       issue(bufs[ST - 1], s0 + ST - 1, s0 + ST - 1 < whole);
-    } else if (first) {
+    } else if (first && s0 + ST - 1 < whole) {
       lin_wait<(ST - 1) * LPS>();
     } else {
-      lin_wait<0>();  // (after a first tile the counter holds its stores too)
+      lin_wait<0>();  // (loads of no lanes are not relied on to count; after a first tile the counter holds its stores)
     }
     // Step s: an operand set is read while the one before is multiplied.  Before the last set's MFMAs every operand of
     // the step is in registers: the workgroup meets, and the step's buffer takes step s + ST, half of its loads among
@@ -437,7 +437,8 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a) {
                 LPS / 2, LPS);
 #pragma unroll
           for (int kk = 1; kk + 1 < KK; ++kk) phase(kk, bufs[u], kk + 1, nullptr, 0, 0, 0, 0);
-          lin_wait<(ST - 2) * LPS>();
+          if (now + ST - 1 < whole) lin_wait<(ST - 2) * LPS>();
+          else lin_wait<0>();
           phase(KK - 1, bufs[(u + 1) % ST], 0, bufs[u], now + ST, now + ST < whole ? -1 : 0, 0, LPS / 2);
         }
       }

@@ -236,7 +236,13 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_quant_kerne
     }
   } else {
     for (int64_t k0 = t * 8; k0 < a.k; k0 += THREADS * 8) {
-      row_values<OP, T, false>(a, row, (int)k0, y[0], ss, false);
+      RowArgs b = a;
+      if (OP == NORM && a.r) {  // (this thread's own sums, as written: x and the residual may be gone, if they lie there)
+        b.x = a.hidden;
+        b.ldx = a.ldh;
+        b.r = nullptr;
+      }
+      row_values<OP, T, false>(b, row, (int)k0, y[0], ss, false);
       put(y[0], (int)k0);
     }
   }

@@ -170,8 +170,10 @@ class _Part(torch.nn.Module):
             x = _Codes(*linear.quantize_rows(x))
         if x.parts is None:
             x.parts = self.fused(x.codes, x.scales).split(self.sizes, -1)
-        # (dense, as a Linear of its own leaves it: the decode cache takes K and V at the same strides)
-        return x.parts[self.index].contiguous()
+        part = x.parts[self.index]
+        # (V dense, as a Linear of its own leaves it and the rotary embedding leaves Q and K: the decode cache takes K and V
+        # at the same strides)
+        return part.contiguous() if self.index == 2 else part
 
 
 def _int8_layer_forward(self, hidden_states, **kwargs):
@@ -202,6 +204,7 @@ def use_int8_layers(model, lm_head=False):
     if model.training:
         raise ValueError("8-bit layers are for inference: call model.eval() first")
     head = model.get_output_embeddings() if lm_head else None
+    kinds = set()
     for layer in layers:
         attention, mlp = layer.self_attn, layer.mlp
         if isinstance(attention.q_proj, _Part):
@@ -212,8 +215,11 @@ def use_int8_layers(model, lm_head=False):
                   mlp.down_proj) + ((head,) if lm_head else ()):
             if type(l) is not torch.nn.Linear:
                 raise ValueError(f"8-bit layers are made from torch.nn.Linear, not {type(l).__name__}")
+            kinds.add((l.weight.device.type, l.weight.dtype))
         if mlp.gate_proj.out_features != mlp.up_proj.out_features:
             raise ValueError("gate and up projections of different widths")
+    if len(kinds) > 1:
+        raise ValueError(f"8-bit layers are made from weights of one type on one kind of device, not {sorted(map(str, kinds))}")
     for layer in layers:
         attention, mlp = layer.self_attn, layer.mlp
         projections = (attention.q_proj, attention.k_proj, attention.v_proj)
