@@ -217,7 +217,11 @@ def operands(seed, m, n, k, dtype, bias, residual):
 LINEAR = [(1, 1, 1), (1, 5, 15), (1, 4608, 3584), (2, 17, 16), (3, 64, 100), (4, 100, 1000), (5, 9, 127), (8, 513, 2049),
           (9, 1, 129), (9, 64, 128), (16, 63, 1000), (16, 200, 8192), (17, 65, 257), (32, 100, 4100), (33, 64, 64),
           (33, 40, 30000), (64, 130, 1), (64, 3, 2048), (65, 128, 100), (100, 300, 4097), (129, 127, 513), (257, 200, 384),
-          (300, 1000, 640), (513, 2, 255), (2, 300, 131071), (70, 40, 20001)]
+          (300, 1000, 640), (513, 2, 255), (2, 300, 131071), (70, 40, 20001),
+          # few rows, where waves share K: fewer steps than waves, as many, one more; channels that end inside a block
+          (1, 1283, 5120), (1, 20001, 300), (2, 20010, 1025), (3, 8192, 1000), (4, 30, 128), (7, 4611, 1024), (8, 700, 12000),
+          (12, 20001, 640), (16, 9, 130), (16, 5120, 1152), (20, 5123, 1280), (24, 2000, 2048), (31, 513, 3584), (32, 17, 40),
+          (17, 20001, 513), (30, 1000, 30001)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEAR)
@@ -231,6 +235,14 @@ def test_int8_linear(module, m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(2048, 4100, 300), (4100, 4097, 129), (8192, 2304, 256)])
 def test_int8_linear_many_tiles(module, m, n, k):
+    x, xs, w, ws, b, r = operands(m, m, n, k, torch.bfloat16, True, True)
+    check_linear(x, xs, w, ws, b, r, torch.bfloat16, Q.int8_linear(x, xs, w, ws, b, r))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 12500, 4000), (2, 12501, 4001), (3, 40001, 2600), (16, 30003, 3400), (17, 40001, 2600),
+                                   (32, 30003, 3400)])
+def test_few_rows_of_many_weights(module, m, n, k):
+    """Products whose weights are loaded past the caches, and short of that."""
     x, xs, w, ws, b, r = operands(m, m, n, k, torch.bfloat16, True, True)
     check_linear(x, xs, w, ws, b, r, torch.bfloat16, Q.int8_linear(x, xs, w, ws, b, r))
 

@@ -1068,7 +1068,7 @@ int tri_int8_linear(const int8_t* x, int64_t ldx, const float* xs, const int8_t*
       return fail("int8_linear: workspace too small (%lld bytes needed)", (long long)(p.splits * m * n * 4));
     a.part = static_cast<int32_t*>(workspace);
   }
-  if (p.kind && ((m + p.bm - 1) / p.bm) * ((n + p.bn - 1) / p.bn) > (1 << 22))
+  if (p.kind <= 6 && ((m + p.bm - 1) / p.bm) * ((n + p.bn - 1) / p.bn) > (1 << 22))
     return fail("int8_linear: too many outputs for one call");
   a.x = x;
   a.ldx = ldx;

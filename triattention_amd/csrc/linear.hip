@@ -2,10 +2,13 @@
 // x [M][K] and w [N][K] int8 rows, int32 sums (exact: K <= 131071 keeps 128 * 128 * K below 2^31), the epilogue in fp32,
 // one rounding to the output's type.
 //
-// dot_kernel, up to 4 rows of x: the work is the stream of w.  A wave reads 8 rows x 128 bytes per load (8 lanes a row,
+// dot_kernel, up to 2 rows of x: the work is the stream of w.  A wave reads 8 rows x 128 bytes per load (8 lanes a row,
 // whole cache lines), takes v_dot4_i32_i8 against the rows of x, and the waves of a workgroup share the K axis.  (16 rows x
 // 64 bytes, the MFMA's own operand order, streams at 0.7 of that rate.)  1 row x 152,064 channels x 3,584: 77 us, 7.0 TB/s;
-// x 3,584 x 18,944: 11.8 us, 5.8 TB/s.
+// x 3,584 x 18,944: 12.3 us, 5.5 TB/s.
+//
+// waves_kernel, up to 32 rows: MFMAs, the K axis shared by the waves of a workgroup, each with buffers of its own.  8 rows x
+// 3,584 channels x 18,944: 11.8 us, 5.8 TB/s; x 152,064 x 3,584: 84 us, 6.5 TB/s.
 //
 // tile_kernel, BM x BN outputs per workgroup: both operands go to LDS 128 bytes of K a step by direct loads (8 rows x 128
 // bytes per wave and load) into two to four buffers, awaited by count, so that one to three steps are in flight.
@@ -274,17 +277,121 @@ __device__ __forceinline__ v4i lin_rsrc(const void* p) {
 // kernels uses m0.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+template <bool STREAM = false>
 __device__ __forceinline__ void lin_lds_load(v4i rsrc, int off, int soff, uint32_t dst, int mask) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\ts_nop 2\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
-      "s_mov_b64 exec, -1" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
-      "v"(off), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soff)),
-      "s"(__builtin_amdgcn_readfirstlane(mask))
-      : "memory", "m0");
+  const uint32_t to = __builtin_amdgcn_readfirstlane(dst);
+  soff = __builtin_amdgcn_readfirstlane(soff);
+  mask = __builtin_amdgcn_readfirstlane(mask);
+#define LIN_LOAD(policy)                                                                                      \
+  asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\ts_nop 2\n\t"               \
+               "buffer_load_dwordx4 %1, %2, %3 offen " policy "lds\n\ts_mov_b64 exec, -1" ::"s"(to), "v"(off), \
+               "s"(rsrc), "s"(soff), "s"(mask)                                                                \
+               : "memory", "m0")
+  if constexpr (STREAM) LIN_LOAD("nt ");
+  else LIN_LOAD("");
+#undef LIN_LOAD
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t lin_lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// Up to MT * 16 rows: MT x NT blocks of 16 rows by 16 channels per workgroup, whose waves share the K axis.  Wave w takes
+// steps w, w + WAVES, ... through ST buffers of its own, so that nothing in the loop waits for another wave; their sums
+// meet in LDS.  STREAM: the weights' loads are non-temporal.  Against tile_kernel's meetings at every step, and its splits' second launch: 8 rows x 3,584 channels x
+// 18,944 11.8 us (5.8 TB/s) against 15.8, 16 x 4,608 x 3,584 6.1 against 7.9, 8 x 640 x 12,000 6.4 against 9.5.
+template <int MT, int NT, int WAVES, int ST, bool STREAM>
+__device__ __forceinline__ void linear_waves(const LinearArgs& a) {
+  constexpr int LPS = 2 * (MT + NT), BUF = LPS * 1024;  // loads (8 rows each) and bytes of a step
+  __shared__ __align__(16) int8_t bufs[WAVES][ST][BUF];
+  __shared__ __align__(16) int red[WAVES][MT][NT * 16][16];
+  const int L = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * (NT * 16);
+  const int steps = (a.k + LIN_KS - 1) / LIN_KS, full = a.k / LIN_KS, last_chunk = (a.k - 1) & ~15;
+  const int mine = (steps - wave + WAVES - 1) / WAVES;  // (steps >= 1; none for the last waves of a short row)
+  const v4i rx = lin_rsrc(a.x), rw = lin_rsrc(a.w + (int64_t)n0 * a.ldw);
+  const int chunk = (L & 7) ^ (L >> 3);
+  int vx[2 * MT], vw[2 * NT];
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) vx[i] = min(i * 8 + (L >> 3), a.m - 1) * (int)a.ldx;
+#pragma unroll
+  for (int i = 0; i < 2 * NT; ++i) vw[i] = min(i * 8 + (L >> 3), a.n - 1 - n0) * (int)a.ldw;
+  auto issue = [&](int u, int i) __attribute__((always_inline)) {  // this wave's step i into buffer u
+    const int s = wave + i * WAVES, mask = i < mine ? -1 : 0;
+    const int koff = min(s * LIN_KS + chunk * 16, last_chunk) - s * LIN_KS;
+    const uint32_t dst = lin_lds_addr(bufs[wave][u]);
+#pragma unroll
+    for (int p = 0; p < 2 * NT; ++p) lin_lds_load<STREAM>(rw, vw[p] + koff, s * LIN_KS, dst + p * 1024, mask);
+#pragma unroll
+    for (int p = 0; p < 2 * MT; ++p) lin_lds_load(rx, vx[p] + koff, s * LIN_KS, dst + (2 * NT + p) * 1024, mask);
+  };
+  const int lr = L & 15, lc = L >> 4, sw = lr & 7;
+  v4i acc[NT][MT] = {};
+#pragma unroll
+  for (int u = 0; u < ST; ++u) issue(u, u);
+  for (int i = 0; i < mine; i += ST) {
+#pragma unroll
+    for (int u = 0; u < ST; ++u) {
+      if (i + u < mine) {
+        if (i + u + ST - 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * LPS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const int s = wave + (i + u) * WAVES;
+        v4i fw[2][NT], fx[2][MT];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const int slot = ((kk * 4 + lc) ^ sw) * 16;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            fw[kk][n] = *reinterpret_cast<const v4i*>(bufs[wave][u] + (n * 16 + lr) * LIN_KS + slot);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            fx[kk][m] = *reinterpret_cast<const v4i*>(bufs[wave][u] + ((NT + m) * 16 + lr) * LIN_KS + slot);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the operands are in registers: the buffer is free
+        issue(u, i + u + ST);
+        if (s >= full) {
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) fx[kk][m] = lin_mask(fx[kk][m], a.k - s * LIN_KS - (kk * 4 + lc) * 16);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[n][m] = MfmaI8<16>::run(fw[kk][n], fx[kk][m], acc[n][m]);
+      }
+    }
+  }
+  // (a lane's column of a block is a row of x, its rows four channels)
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[wave][m][n * 16 + 4 * lc + e][lr] = acc[n][m][e];
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * NT * 256; o += WAVES * 64) {
+    const int n = n0 + o % (NT * 16), m = o / (NT * 16);
+    if (m >= a.m || n >= a.n) continue;
+    int one[1] = {0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) one[0] += red[w][m >> 4][n - n0][m & 15];
+    lin_typed<false>(a, LIN_EDGE, [&](auto type, auto, auto res) {
+      using T = decltype(type);
+      float ws[1], bias[1];
+      T r[1];
+      lin_channels<T, false>(a, 0, n, ws, bias);
+      if constexpr (decltype(res)::value) lin_residual<T, false>(a, m, 0, n, r);
+      lin_out<T, false, decltype(res)::value>(a, m, 0, 0, n, a.xs[m], ws, bias, r, one);
+    });
+  }
+}
+
+template <int MT, int NT, int WAVES, int ST, bool STREAM>
+__global__ __launch_bounds__(WAVES * 64) void waves_kernel(LinearArgs a) {
+  linear_waves<MT, NT, WAVES, ST, STREAM>(a);
 }
 
 // WM x WN waves, S x S MFMA blocks, ST buffers of 128 bytes of K.  Workgroup w takes tiles w, w + gridDim.x, ...: with
@@ -590,7 +697,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 }
 
 // ------------------------------------------------------------------ launches
-// How one product is cut: `kind` 0 the dot kernel, otherwise a tile form; splits of `per` steps each.
+// How one product is cut: `kind` 0 the dot kernel, 1 to 6 a tile form, from 7 a form of waves_kernel; splits of `per`
+// steps each.
 struct LinearPlan {
   int kind, bm, bn, splits, per;
   int groups;  // workgroups, at most one a tile
@@ -609,39 +717,67 @@ constexpr LinearForm LIN_FORMS[] = {
     {256, 256, 1, 1.0, 5.5},
 };
 
+// The forms of waves_kernel (rows and channels in blocks of 16).
+struct LinearWaves {
+  int mt, nt, waves, resident;
+  double step, fixed;
+};
+constexpr LinearWaves LIN_WAVES[] = {
+    {1, 1, 8, 2, 0.59, 0.4}, {1, 2, 8, 1, 0.85, 0.6}, {1, 2, 4, 2, 0.52, 0.5}, {2, 1, 8, 1, 0.74, 0.85}, {2, 2, 4, 2, 0.7, 0.6},
+};
+
+// Weights past the caches: above 100 MB of w few calls find it in the last-level cache (256 MB, shared with all else), and
+// non-temporal loads win (8 rows x 152,064 channels x 3,584 84 us against 94, x 37,888 x 3,584 24.1 against 26.4); below they
+// lose what repeated calls find there (x 3,584 x 18,944 18.7 against 15.0).
+constexpr bool linear_streams(int n, int k) { return (int64_t)n * k >= 100000000; }
+
+// us of `work` workgroups that take `per` turns of `step` us alone and `load` us of their CU's data path each
+inline double linear_rounds(int64_t work, int cus, int resident, int per, double step, double load, double fixed) {
+  const int64_t slots = (int64_t)cus * resident, rounds = work / slots;
+  const int left = (int)((work - rounds * slots + cus - 1) / cus);
+  double t = rounds * (per * std::max(step, resident * load) + fixed);
+  if (left) t += per * std::max(step, left * load) + fixed;
+  return t;
+}
+
 // The form and the split that this model of their time holds fastest: rounds of resident workgroups, each step bound by
 // its own latency, by the bytes that a CU takes from its L2 (64.7 GB/s) or by the matrix cores (9.8 Top/s a CU); never
 // below the stream of both operands (6 TB/s); a split adds its launch and its partials' way through memory.  Fitted to
 // 2,700 timings of 149 shapes (5 to 8,192 rows, 640 to 37,888 channels, K 1,000 to 18,944): its choice takes 0.2% more
 // than the fastest of all forms and splits on the mean, 5% at most.
+// Up to 32 rows the forms that share K inside a workgroup stand beside them (70 GB/s a CU, fitted to 2,800 timings of 181
+// shapes: 2% more than the fastest on the mean).
 inline LinearPlan linear_plan(int m, int n, int k, int cus) {
   const int steps = (k + LIN_KS - 1) / LIN_KS;
+  // One or two rows against many weights: v_dot4 keeps up with the stream and loads past the caches (1 row x 152,064
+  // channels x 3,584 78.6 us against 88 by MFMAs, x 8,192 x 8,192 11.0 against 12.6; x 4,096 x 4,096 5.0 either way, x 2,048 x
+  // 2,048 3.7 against 2.9; 4 rows x 37,888 x 3,584 27.4 against 25.6).
+  if (m <= 2 && (int64_t)n * k >= 45000000) return {0, m, 16, 1, steps, INT32_MAX};
   LinearPlan best{};
-  best.splits = 1;
-  best.per = steps;
-  // Up to 4 rows v_dot4 keeps up with the stream (K 18,944 x 3,584 channels: 11.8 / 12.5 / 15.5 us for 1 / 2 / 4 rows, 23
-  // for 8; the 16-row tile 15-16 us at any count).
-  if (m <= 4) return best;
   double least = 1e300;
   const double stream = ((double)n * k + (double)m * k) / 6.0e6;
+  auto consider = [&](double t, const LinearPlan& p) {
+    if (t < least) least = t, best = p;
+  };
   for (int f = 0; f < 6; ++f) {
     const LinearForm& form = LIN_FORMS[f];
     const int64_t tiles = (int64_t)((m + form.bm - 1) / form.bm) * ((n + form.bn - 1) / form.bn);
-    const int64_t slots = (int64_t)cus * form.resident;
-    const double bytes = (form.bm + form.bn) * LIN_KS / 64.7e3, ops = 2.0 * form.bm * form.bn * LIN_KS / 9.8e6;
+    const double load = std::max((form.bm + form.bn) * LIN_KS / 64.7e3, 2.0 * form.bm * form.bn * LIN_KS / 9.8e6);
     for (int want = 1; want <= 16 && (want == 1 || (steps >= 4 * want && tiles * want <= 5 * (int64_t)cus)); ++want) {
       const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
-      const int64_t work = tiles * splits, rounds = work / slots;
-      const int left = (int)((work - rounds * slots + cus - 1) / cus);
-      double t = rounds * (per * std::max(form.step, form.resident * std::max(bytes, ops)) + form.fixed);
-      if (left) t += per * std::max(form.step, left * std::max(bytes, ops)) + form.fixed;
-      t = std::max(t, stream);
+      double t = std::max(stream, linear_rounds(tiles * splits, cus, form.resident, per, form.step, load, form.fixed));
       if (splits > 1) t += 2.6 + 0.44 * splits + 8.0 * splits * m * n / 3.77e6;
-      if (t < least) {
-        least = t;
-        best = {f + 1, form.bm, form.bn, splits, per, INT32_MAX};
-      }
+      consider(t, {f + 1, form.bm, form.bn, splits, per, INT32_MAX});
     }
+  }
+  for (int f = 0; f < 5; ++f) {
+    const LinearWaves& form = LIN_WAVES[f];
+    if (m > 16 * form.mt) continue;
+    const double load = form.waves * 16 * (form.mt + form.nt) * LIN_KS / 70e3;
+    const int per = (steps + form.waves - 1) / form.waves, bn = 16 * form.nt;
+    const double least_us = linear_streams(n, k) && bn == 32 && form.waves == 4 ? 0.92 * stream : stream;
+    consider(std::max(least_us, linear_rounds((n + bn - 1) / bn, cus, form.resident, per, form.step, load, form.fixed)),
+             {f + 7, 16 * form.mt, bn, 1, steps, INT32_MAX});
   }
   // (the largest form's workgroups take tile after tile; a multiple of the XCDs keeps a workgroup's tiles on its XCD)
   if (best.kind == 6) best.groups = std::max(8, cus & ~7);
@@ -655,18 +791,28 @@ inline void launch_tile(const LinearArgs& a, int groups, hipStream_t s) {
   else tile_kernel<BM, BN, WM, WN, S, ST, false><<<grid, block, 0, s>>>(a);
 }
 
-template <int MR, int U>
+template <int MT, int NT, int WAVES, int ST, bool STREAM = false>
+inline void launch_waves(const LinearArgs& a, hipStream_t s) {
+  waves_kernel<MT, NT, WAVES, ST, STREAM><<<dim3((a.n + NT * 16 - 1) / (NT * 16)), dim3(WAVES * 64), 0, s>>>(a);
+}
+
+template <int MR>
 inline void launch_dot(const LinearArgs& a, hipStream_t s) {
-  constexpr int NR = 2, WAVES = 8;
+  constexpr int NR = 2, WAVES = 8, U = 4;
   dot_kernel<MR, NR, WAVES, U><<<dim3((a.n + NR * 8 - 1) / (NR * 8)), dim3(WAVES * 64), 0, s>>>(a);
 }
 
 inline void launch_linear(LinearArgs a, const LinearPlan& p, hipStream_t s) {
-  if (p.kind == 0) {
-    if (a.m == 1) launch_dot<1, 4>(a, s);
-    else if (a.m == 2) launch_dot<2, 4>(a, s);
-    else launch_dot<4, 2>(a, s);
-    return;
+  switch (p.kind) {
+    case 0:
+      if (a.m == 1) launch_dot<1>(a, s);
+      else launch_dot<2>(a, s);
+      return;
+    case 7: return launch_waves<1, 1, 8, 2>(a, s);
+    case 8: return launch_waves<1, 2, 8, 2>(a, s);
+    case 9: return linear_streams(a.n, a.k) ? launch_waves<1, 2, 4, 3, true>(a, s) : launch_waves<1, 2, 4, 3>(a, s);
+    case 10: return launch_waves<2, 1, 8, 3>(a, s);
+    case 11: return linear_streams(a.n, a.k) ? launch_waves<2, 2, 4, 2, true>(a, s) : launch_waves<2, 2, 4, 2>(a, s);
   }
   a.tiles_m = (a.m + p.bm - 1) / p.bm;
   a.tiles_n = (a.n + p.bn - 1) / p.bn;

@@ -126,7 +126,7 @@ def int8_linear(codes, scales, weight, weight_scales, bias=None, residual=None, 
     module._check_linear(x, scales, weight, weight_scales, bias, other, out_dtype)
     out = codes.new_empty(shape, dtype=out_dtype)
     m = x.size(0)
-    size = module.int8_linear_workspace(m, n, k, codes.device) if m > 4 else 0  # (fewer rows are never split over K)
+    size = module.int8_linear_workspace(m, n, k, codes.device) if m else 0
     workspace = codes.new_empty(size, dtype=torch.uint8) if size else None
     module._int8_linear(x, scales, weight, weight_scales, bias, other, out, n, workspace)
     return out
