@@ -728,7 +728,7 @@ constexpr LinearWaves LIN_WAVES[] = {
 
 // Weights past the caches: above 100 MB of w few calls find it in the last-level cache (256 MB, shared with all else), and
 // non-temporal loads win (8 rows x 152,064 channels x 3,584 84 us against 94, x 37,888 x 3,584 24.1 against 26.4); below they
-// lose what repeated calls find there (x 3,584 x 18,944 18.7 against 15.0).
+// gain less (x 3,584 x 18,944 13.3 against 14.0) than they lose where calls do find it there (13.1 against 11.8).
 constexpr bool linear_streams(int n, int k) { return (int64_t)n * k >= 100000000; }
 
 // us of `work` workgroups that take `per` turns of `step` us alone and `load` us of their CU's data path each
@@ -749,10 +749,11 @@ inline double linear_rounds(int64_t work, int cus, int resident, int per, double
 // shapes: 2% more than the fastest on the mean).
 inline LinearPlan linear_plan(int m, int n, int k, int cus) {
   const int steps = (k + LIN_KS - 1) / LIN_KS;
-  // One or two rows against many weights: v_dot4 keeps up with the stream and loads past the caches (1 row x 152,064
-  // channels x 3,584 78.6 us against 88 by MFMAs, x 8,192 x 8,192 11.0 against 12.6; x 4,096 x 4,096 5.0 either way, x 2,048 x
-  // 2,048 3.7 against 2.9; 4 rows x 37,888 x 3,584 27.4 against 25.6).
-  if (m <= 2 && (int64_t)n * k >= 45000000) return {0, m, 16, 1, steps, INT32_MAX};
+  // One or two rows against many weights: v_dot4 keeps up with the stream and loads past the caches.  1 row x 152,064 channels
+  // x 3,584 78.6 us against 88 by MFMAs; weights in no cache: x 37,888 x 3,584 22.4 against 25.3, x 8,192 x 8,192 11.8 against
+  // 14.2, x 3,584 x 3,584 4.3 against 4.8, x 2,048 x 2,048 3.7 either way (and 3.7 against 2.9 with them there).  Fewer
+  // channels leave CUs without work; 4 rows x 37,888 x 3,584 27.4 against 25.6.
+  if (m <= 2 && n >= 2048 && (int64_t)n * k >= 12000000) return {0, m, 16, 1, steps, INT32_MAX};
   LinearPlan best{};
   double least = 1e300;
   const double stream = ((double)n * k + (double)m * k) / 6.0e6;
