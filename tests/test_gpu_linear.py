@@ -10,6 +10,8 @@ additions round five times in fp32 (2^-24 of the terms' magnitudes each), and th
 half of fp16's smallest step)."""
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -304,6 +306,45 @@ def test_strided_and_repeated_codes(module):
         xs = torch.rand(rows.size(0), generator=g, device=DEV)
         out = Q.int8_linear(rows, xs, w, ws, out_dtype=torch.float32)
         check_linear(rows, xs, w, ws, None, None, torch.float32, out)
+
+
+def test_a_layer_moved_and_copied(module):
+    """Weights of 100 input channels (rows padded to 112 bytes) through the host and a deep copy."""
+    torch.manual_seed(5)
+    layer = torch.nn.Linear(100, 24).to(DEV, torch.bfloat16)
+    layer = Q.Int8Linear(layer)
+    x = torch.randn(3, 100, dtype=torch.bfloat16, device=DEV)
+    with torch.no_grad():
+        want = layer(x)
+        assert torch.equal(copy.deepcopy(layer)(x), want)
+        assert torch.equal(layer.cpu().to(DEV)(x), want)
+
+
+def test_offsets_past_32_bits(module):
+    """70,000 rows of 32,768: the last rows come out as they do alone (codes and integer sums are the same bits)."""
+    m, k, tail = 70000, 32768, slice(-40, None)
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=DEV).normal_(generator=gen(9))
+    codes, scales = Q.quantize_rows(x)
+    for whole, alone in zip((codes, scales), Q.quantize_rows(x[tail])):
+        assert torch.equal(whole[tail], alone)
+    w = torch.ones(k, dtype=torch.bfloat16, device=DEV)
+    for whole, alone in zip(Q.rms_norm_quant(x, w, 1e-6, residual=x), Q.rms_norm_quant(x[tail], w, 1e-6, residual=x[tail])):
+        assert torch.equal(whole[tail], alone)
+    for whole, alone in zip(Q.silu_mul_quant(x, x), Q.silu_mul_quant(x[tail], x[tail])):
+        assert torch.equal(whole[tail], alone)
+    del x, whole, alone
+    # codes, then weights, then outputs and residual of more than 2^31 elements
+    out = Q.int8_linear(codes, scales, codes[:300], scales[:300])
+    assert torch.equal(out[tail], Q.int8_linear(codes[tail], scales[tail], codes[:300], scales[:300]))
+    for rows in (1, 8, 32, 300):
+        out = Q.int8_linear(codes[:rows], scales[:rows], codes, scales)
+        assert torch.equal(out[:, tail], Q.int8_linear(codes[:rows], scales[:rows], codes[tail], scales[tail]))
+    few = codes[:, :128]
+    out = Q.int8_linear(few, scales, few[:k], scales[:k])
+    assert torch.equal(out[tail], Q.int8_linear(few[tail], scales[tail], few[:k], scales[:k]))
+    out = Q.int8_linear(few, scales, few[:k], scales[:k], residual=out)
+    assert torch.equal(out[tail, :100], Q.int8_linear(few[tail], scales[tail], few[:100], scales[:100],
+                                                      residual=Q.int8_linear(few[tail], scales[tail], few[:100], scales[:100])))
 
 
 def test_no_rows(module):

@@ -162,6 +162,15 @@ class Int8Linear(torch.nn.Module):
         self.register_buffer("scales", scales)
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, recurse=True):
+        """Moves keep the codes' rows at multiples of 16 bytes (a copy of a row-padded tensor is dense)."""
+        super()._apply(fn, recurse)
+        n, k = self.codes.shape
+        if self.codes.stride(0) % 16:
+            codes = self.codes.new_empty((n, k + -k % 16))[:, :k]
+            self.codes = codes.copy_(self.codes)
+        return self
+
     def forward(self, x, scales=None, residual=None):
         if scales is None:
             x, scales = quantize_rows(x)
